@@ -233,6 +233,70 @@ int nmt_sdpa_decode_bf16(const void* Q, void* K_cache, void* V_cache, void* O, c
                          int64_t S_cache, int64_t total_S, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                          void* workspace, void* stream);
 
+/* ---- Attention over a paged key-value cache and over whole prompts ----------------- */
+
+/* The cache of several sequences, cut into pages.  A page holds page_size consecutive positions of ONE sequence for every
+ * kv head, [kv_heads][page_size][head_dim] contiguous - each page is a small cache of the layout nmt_sdpa_decode_bf16
+ * reads - and pages lie k_page_stride / v_page_stride elements apart (so K and V may share one allocation).  Position s
+ * of sequence b is row s % page_size of page page_table[b][s / page_size].  These entry points have no counterpart in
+ * the reference, whose cache is one contiguous buffer for one sequence (tensor layout of ops/attention/sdpa_decode.cuh).
+ *   page_size  a power of two, 8 .. 1024;  head_dim 64 or 128;  k, v 16-byte aligned, page strides multiples of 16 bytes
+ *   dtype      NMT_CACHE_BF16, or NMT_CACHE_E4M3: an element stands for its value times the scale
+ *   k_scale, v_scale   device fp32, scale_count of them: 1 (per tensor) or kv_heads; NULL = 1.0
+ *   page_table device int32 [batch][max_pages];  seq_lens device int32 [batch]: tokens of each sequence, the ones that
+ *              the call appends included.  Both are read by the kernels, not by the host: a captured graph may be replayed
+ *              with other contents.
+ * A page id outside [0, num_pages) is never dereferenced, a length is taken as at most max_pages * page_size. */
+#define NMT_CACHE_BF16 0
+#define NMT_CACHE_E4M3 1
+typedef struct nmt_paged_cache {
+    void* k;
+    void* v;
+    int64_t k_page_stride, v_page_stride;   /* elements between two pages */
+    int64_t num_pages, page_size, kv_heads, head_dim;
+    int64_t dtype;
+    const float* k_scale;
+    const float* v_scale;
+    int64_t scale_count;
+    const int32_t* page_table;
+    const int32_t* seq_lens;
+    int64_t batch, max_pages;
+} nmt_paged_cache;
+
+/* Writes the keys and values of `tokens` new tokens into their pages, and rotates K (and Q) by position on the way.
+ *   cu_new     device int32 [batch + 1], ascending: the tokens of sequence b are rows cu_new[b] .. cu_new[b + 1] - 1 of k,
+ *              v and q, and its LAST one has position seq_lens[b] - 1.  Rows behind cu_new[batch] are padding: not read,
+ *              nothing written for them.  NULL: one token per sequence (tokens == batch), the decode step.
+ *   k, v       bf16 [tokens][kv_heads][head_dim] with any token and head strides (in elements, multiples of 8)
+ *   rope       NULL: no rotation.  Else fp32 [rope_rows][rot_dim]: row p holds rot_dim / 2 cosines, then as many sines, of
+ *              position p.  The first rot_dim entries of every head are turned in pairs, (a, b) -> (a cos - b sin,
+ *              b cos + a sin): entries (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved != 0.  rot_dim % 16 == 0.
+ *   q, q_out   bf16 [tokens][q_heads][head_dim], or both NULL; needs rope.  q_out may be q.
+ * fp32 arithmetic, one rounding to the type that is stored; e4m3(x / scale) saturates at +-448, NaN stays NaN.
+ * A token whose position, page id or rope row is out of range writes nothing and sets *err_flag (device int32, may be
+ * NULL) to 1.  Two tokens never share a slot unless the page table makes two sequences share a page; then which of
+ * them stays is undefined.  tokens == 0 is a no-op.  One launch. */
+int nmt_kv_append_paged_bf16(const nmt_paged_cache* cache, const int32_t* cu_new, int64_t tokens, const void* k,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                             int64_t v_head_stride, const float* rope, int64_t rope_rows, int64_t rot_dim, int interleaved,
+                             const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, void* q_out,
+                             int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t* err_flag, void* stream);
+
+/* Attention of ONE new token per sequence over its pages (the new token's own key and value among them, once
+ * nmt_kv_append_paged_bf16 has put them there):
+ *   out[b, h] = sum_s softmax_s(scale * q[b, h] . K[b, g, s]) V[b, g, s],  s < seq_lens[b],  g = h / (heads / kv_heads)
+ * q, out bf16 [batch][heads][head_dim] with any sequence and head strides (elements, multiples of 8; out may be q).
+ * heads a multiple of kv_heads; scale positive and finite.  fp32 scores, softmax statistics and sums; bf16 weights are
+ * carried in two terms (16 significant bits), e4m3 caches are multiplied as f16, exactly.  A sequence of length 0 gives
+ * zeros.  Rows at or past a sequence's length are never used, whatever they hold.  A page id outside [0, num_pages)
+ * reads as zeros and sets *err_flag (device int32, may be NULL) to 1; so does a length past max_pages * page_size.
+ * workspace: nmt_sdpa_decode_paged_workspace_bytes(...) bytes, 16-byte aligned, no initialisation; calls whose kernels
+ * may overlap need one each.  The split of the work depends on the lengths alone, so results repeat bit for bit.  Two launches. */
+int64_t nmt_sdpa_decode_paged_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim);
+int nmt_sdpa_decode_paged_bf16(const nmt_paged_cache* cache, const void* q, int64_t q_seq_stride, int64_t q_head_stride, void* out,
+                               int64_t out_seq_stride, int64_t out_head_stride, int64_t heads, float scale, int32_t* err_flag,
+                               void* workspace, void* stream);
+
 /* fp32 twin, unsplit; replaces causal_conv1d_prefill_fp32 (ops/mamba2/causal_conv1d.cuh:115-127). */
 int nmt_causal_conv1d_silu_f32(const float* x, const float* w, const float* bias, float* y, float* state_out,
                                int64_t conv_dim, int64_t S, int64_t batch, void* stream);

@@ -17,6 +17,16 @@ _i64 = C.c_int64
 _f = C.c_float
 _int = C.c_int
 
+
+class PagedCache(C.Structure):
+    """nmt_paged_cache of include/nemotron_b200.h, field by field."""
+    _fields_ = [("k", _p), ("v", _p), ("k_page_stride", _i64), ("v_page_stride", _i64), ("num_pages", _i64), ("page_size", _i64),
+                ("kv_heads", _i64), ("head_dim", _i64), ("dtype", _i64), ("k_scale", _p), ("v_scale", _p), ("scale_count", _i64),
+                ("page_table", _p), ("seq_lens", _p), ("batch", _i64), ("max_pages", _i64)]
+
+
+_cache = C.POINTER(PagedCache)
+
 # name -> (restype, argtypes); mirrors include/nemotron_b200.h declaration by declaration.
 PROTOTYPES = {
     "nmt_version": (C.c_char_p, []),
@@ -39,6 +49,10 @@ PROTOTYPES = {
     "nmt_gemv_w8a16_gated": (_int, [_p, _p, _p, _f, _i64, _p, _p, _p, _p, _i64, _i64, _p]),
     "nmt_sdpa_decode_workspace_bytes": (_i64, [_i64, _i64]),
     "nmt_sdpa_decode_bf16": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p]),
+    "nmt_kv_append_paged_bf16": (_int, [_cache, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _int, _p, _i64, _i64, _i64, _p, _i64, _i64,
+                                        _p, _p]),
+    "nmt_sdpa_decode_paged_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "nmt_sdpa_decode_paged_bf16": (_int, [_cache, _p, _i64, _i64, _p, _i64, _i64, _i64, _f, _p, _p, _p]),
     "nmt_ssm_decode_step_bf16": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f, _f, _p]),
     "nmt_relu2_f32": (_int, [_p, _p, _i64, _p]),
     "nmt_add_bf16": (_int, [_p, _p, _p, _i64, _p]),

@@ -29,6 +29,7 @@
 #include <cuda.h>
 #include <cuda_fp8.h>
 
+#include "nmt_tensormap.cuh"
 #include "nmt_tma.cuh"
 
 namespace nmt {
@@ -296,21 +297,8 @@ gemv_w8a16_umma_kernel(const __grid_constant__ CUtensorMap wmap, const __nv_bflo
 }
 
 // ---------------------------------------------------------------------------------------------
-// Host side: the tensor map of W (driver entry point fetched at run time; the library does not link libcuda).
+// Host side: the tensor map of W.
 // ---------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
-        return reinterpret_cast<EncodeTiledFn>(p);
-    }();
-    return fn;
-}
-
 int launch_gemv_umma(const void* x, const float* norm_w, float eps, const void* W, const float* w_scale, int activation,
                      const void* residual, void* y, int N, int K, cudaStream_t st) {
     if ((K % 64) != 0 || K > 16384 || (reinterpret_cast<uintptr_t>(x) & 15u)) return NMT_ERR_UNSUPPORTED;

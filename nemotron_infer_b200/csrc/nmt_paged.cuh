@@ -1,0 +1,64 @@
+// What the kernels over a paged key-value cache share: the argument checks and the search for a packed row's sequence.
+#pragma once
+
+#include "nmt_common.cuh"
+
+namespace nmt {
+
+inline bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
+inline int log2_of(int64_t v) { int s = 0; while ((1ll << s) < v) ++s; return s; }
+
+// The cache descriptor on its own: sizes, strides, alignment.  Pointers the kernels need are checked by the callers of
+// this function only where a call has work to do.
+inline int check_paged_cache(const nmt_paged_cache* c) {
+    if (!c) return NMT_ERR_NULL;
+    if (c->batch < 0 || c->max_pages <= 0 || c->num_pages <= 0 || c->kv_heads <= 0 || c->head_dim <= 0) return NMT_ERR_SHAPE;
+    if (c->dtype != NMT_CACHE_BF16 && c->dtype != NMT_CACHE_E4M3) return NMT_ERR_UNSUPPORTED;
+    if ((c->head_dim != 64 && c->head_dim != 128) || !pow2(c->page_size) || c->page_size < 8 || c->page_size > 1024) return NMT_ERR_UNSUPPORTED;
+    if (c->kv_heads > 65535 || c->batch > 0x3fffffff || c->num_pages > 0x7fffffff || c->max_pages > 0x7fffffff / c->page_size) return NMT_ERR_UNSUPPORTED;
+    if ((c->k_scale || c->v_scale) && c->scale_count != 1 && c->scale_count != c->kv_heads) return NMT_ERR_SHAPE;
+    const int64_t page = c->kv_heads * c->page_size * c->head_dim, per16 = c->dtype == NMT_CACHE_BF16 ? 8 : 16;
+    if (c->num_pages > 1 && (c->k_page_stride < page || c->v_page_stride < page)) return NMT_ERR_SHAPE;
+    if (c->num_pages > 1 && (c->k_page_stride > (1ll << 36) || c->v_page_stride > (1ll << 36))) return NMT_ERR_UNSUPPORTED;
+    if (c->num_pages > 1 && (c->k_page_stride % per16 || c->v_page_stride % per16)) return NMT_ERR_ALIGN;
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned4(c->page_table) || !aligned4(c->seq_lens) || !aligned4(c->k_scale) ||
+        !aligned4(c->v_scale))
+        return NMT_ERR_ALIGN;
+    return NMT_OK;
+}
+// A bf16 [tokens][heads][head_dim] view: strides in elements, 16-byte vectors.
+inline int check_view(const void* p, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride) {
+    if (!p) return NMT_ERR_NULL;
+    if (!aligned16(p) || (tokens > 1 && (token_stride & 7)) || (heads > 1 && (head_stride & 7))) return NMT_ERR_ALIGN;
+    if ((tokens > 1 && (token_stride < 0 || token_stride > (1ll << 36))) || (heads > 1 && (head_stride < 0 || head_stride > (1ll << 36))))
+        return NMT_ERR_UNSUPPORTED;
+    return NMT_OK;
+}
+
+// The largest b in [0, n) with cu[b] <= t, or -1; cu ascending.  All 32 lanes probe at once: two rounds of loads for up
+// to 1024 entries instead of ten dependent ones.  Whatever cu holds, only cu[0 .. n - 1] is read and the result is in
+// [-1, n).  Warp-collective.
+__device__ __forceinline__ int find_segment(const int32_t* __restrict__ cu, int n, int t) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = n;
+    while (len > 0) {
+        const int step = (len + 31) >> 5;
+        const int at = lane * step;
+        const bool ok = at < len && cu[lo + at] <= t;
+        const int cnt = __popc(__ballot_sync(0xffffffffu, ok));
+        if (cnt == 0) break;
+        const int skip = (cnt - 1) * step + 1;
+        len = min(step - 1, len - skip);
+        lo += skip;
+    }
+    return lo - 1;
+}
+
+// Two fp32 values -> two e4m3 bytes (`lo` in the low byte): round to nearest even, saturating, NaN kept.
+__device__ __forceinline__ uint32_t e4m3x2_rn(float lo, float hi) {
+    uint32_t r;
+    asm("{ .reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %1, %2; cvt.u32.u16 %0, t; }" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+}  // namespace nmt

@@ -1,0 +1,655 @@
+// Attention of one new token per sequence over a paged key-value cache.
+//
+//   out[b, h] = sum_{s < len_b} p_s V[b, g, s],   p = softmax_s(scale q[b, h] . K[b, g, s]),   g = h / (H_Q / H_KV)
+//
+// Bytes: every cached row once (4 KB per token at 8 heads of 128 in bf16), against 4 flops per query head and byte pair:
+// HBM-bound for every group size there is, so the work is arranged around keeping copies in flight.
+//   * Balance.  A unit is (sequence, kv head, up to 16 of its query heads); it is cut into tiles of 16 KB of K and 16 KB of
+//     V (64 to 256 positions).  All tiles of the batch form one line, sequence by sequence, and each of up to 296 CTAs (two
+//     per SM) takes an equal piece of it, whatever the lengths are: every CTA sums the lengths itself (they are only known
+//     on the device), so a captured graph follows them.  A unit that one CTA holds whole is finished there; a cut one
+//     leaves (maximum, sum, output) per piece in the workspace and a second launch joins the pieces.
+//   * Copies.  A producer warp looks up the pages and brings them in with tensor-map copies (one box per page and 128
+//     bytes of row, swizzled so that ldmatrix reads without bank conflicts) through a ring of three tiles per CTA: 192 KB
+//     per SM on their way.  A page id out of range goes out as a coordinate out of range, which the copy fills with zeros.
+//   * Arithmetic.  Four warps each take every fourth group of 16 positions of a tile and keep their own running maximum, sum
+//     and output, so nothing synchronises inside a unit.  Products run on mma.sync.m16n8k16 with the POSITIONS (K V^T side)
+//     as the 16 rows and up to 8 query heads as the columns: S^T = K Q^T, then O^T = V^T P^T, where P^T comes out of S^T's
+//     registers by an 8x8 register transpose (movmatrix).  The tensor core is fed at one MMA per position and 8 heads -
+//     a tenth of what even this path sustains - so the wider tcgen05 tile would only add its staging (an accumulator in
+//     tensor memory, M = 128 rows for 5 heads) to a kernel that waits for HBM.
+//   * Precision.  P is split into two bf16 terms (p = hi + lo, 16 bits) against a bf16 V.  e4m3 values and the query,
+//     scaled by a power of two per head, are exact in f16 and P keeps 11 bits there.  Scores, maxima, sums, output: fp32.
+#include <cfloat>
+
+#include "nmt_paged.cuh"
+#include "nmt_tensormap.cuh"
+#include "nmt_tma.cuh"
+
+namespace nmt {
+
+NMT_DEFINE_TIMEOUT_READER();
+
+constexpr int kDecWarps = 4;                                       // consumer warps; one more produces
+constexpr int kDecThreads = (kDecWarps + 1) * 32;
+constexpr int kDecStages = 3;
+constexpr int kTileBytes = 16384;                                  // of K, and as much of V
+constexpr int kDecCtas = 2 * kSmCount;
+constexpr int kMergeCols = 68;                                     // 64 columns + 4: head rows of the merge buffer hit different banks
+constexpr size_t kDecMergeBytes = kDecWarps * 8 * kMergeCols * sizeof(float);
+constexpr size_t kDecSmem = 1024 + (size_t)kDecStages * 2 * kTileBytes + kDecMergeBytes;
+
+struct DecodeArgs {
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    int64_t q_ss, q_hs, o_ss, o_hs;
+    const int32_t *seq_lens, *page_table;
+    const float *k_scale, *v_scale;
+    int32_t* err_flag;
+    int4* desc;                                                    // [kDecCtas][2]: what CTA c's piece starts with
+    float2* ml;                                                    // [kDecCtas][2][heads of a unit]: maximum (log 2 units), sum
+    float* o;                                                      // [kDecCtas][2][heads of a unit][D]
+    float scale_log2;
+    int batch, kv_heads, group, chunks, page_shift, max_pages, num_pages, scale_step;
+    int tile_shift;                                                // log2 of positions per tile
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+    uint32_t r;
+    asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(two_bytes));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void tma_page_box(uint32_t smem_dst, const CUtensorMap* map, int x, int row, int head, int page, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Where a CTA stands on the line of tiles.
+struct Cursor {
+    int b, unit, tile, tiles, len;
+    __device__ __forceinline__ void seat(const DecodeArgs& p) {    // length and tile count of sequence b
+        len = b < p.batch ? min(max(p.seq_lens[b], 0), p.max_pages << p.page_shift) : 0;
+        tiles = max(1, (len + (1 << p.tile_shift) - 1) >> p.tile_shift);
+    }
+    __device__ __forceinline__ void next_unit(const DecodeArgs& p) {
+        tile = 0;
+        if (++unit == p.kv_heads * p.chunks) { unit = 0; ++b; seat(p); }
+    }
+};
+
+template <int D, bool E4M3, int NT>                                // NT x 8 query heads per unit
+__global__ void __launch_bounds__(kDecThreads, 2)
+sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const DecodeArgs p) {
+    constexpr int ROWB = D * (E4M3 ? 1 : 2);                       // bytes of a row
+    constexpr int CH = ROWB >= 128 ? 128 : 64;                     // bytes of a swizzled chunk of a row
+    constexpr int NCH = ROWB / CH;
+    constexpr int TK = kTileBytes / ROWB;                          // positions per tile
+    constexpr int STEPS = TK / (16 * kDecWarps);                   // groups of 16 positions a warp takes of a tile
+    constexpr int HPU = NT * 8;
+    constexpr int KS = D / 16;
+    extern __shared__ __align__(1024) uint8_t smem_d[];
+    __shared__ uint64_t s_full[kDecStages], s_empty[kDecStages];
+    __shared__ int64_t s_sum[kDecThreads / 32];
+    __shared__ int64_t s_start[2];                                 // first tile of this CTA, inside sequence s_b
+    __shared__ int s_b;
+    __shared__ float s_m[kDecWarps][HPU], s_l[kDecWarps][HPU];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t ring = (smem_u32(smem_d) + 1023u) & ~1023u;
+    float* merge = reinterpret_cast<float*>(smem_d + (ring - smem_u32(smem_d)) + kDecStages * 2 * kTileBytes);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kDecStages; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_empty[s], kDecWarps); }
+        mbar_init_fence();
+    }
+    pdl_wait();
+    // ---- the line of tiles: total, this CTA's piece, the sequence it starts in ----
+    const int units_per_seq = p.kv_heads * p.chunks;
+    const int per = (p.batch + kDecThreads - 1) / kDecThreads;
+    const int b_lo = min((int)threadIdx.x * per, p.batch), b_hi = min(b_lo + per, p.batch);
+    int64_t mine = 0;
+    bool too_long = false;
+    for (int b = b_lo; b < b_hi; ++b) {
+        const int cap = p.max_pages << p.page_shift, raw = p.seq_lens[b];
+        too_long |= raw > cap;
+        mine += max(1, (min(max(raw, 0), cap) + TK - 1) >> p.tile_shift);
+    }
+    if (too_long && blockIdx.x == 0 && p.err_flag) *p.err_flag = 1;
+    mine *= units_per_seq;
+    int64_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += up;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    int64_t total = 0, before = incl - mine;
+#pragma unroll
+    for (int w = 0; w < kDecThreads / 32; ++w) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
+    }
+    const int ctas = static_cast<int>(min((int64_t)gridDim.x, total));     // every one of them has at least one tile
+    const int64_t begin = (int64_t)blockIdx.x * total / ctas, end = (int64_t)(blockIdx.x + 1) * total / ctas;
+    const bool active = (int)blockIdx.x < ctas;
+    if (active && begin >= before && begin < before + mine) {
+        int64_t at = before;
+        for (int b = b_lo; b < b_hi; ++b) {
+            const int len = min(max(p.seq_lens[b], 0), p.max_pages << p.page_shift);
+            const int64_t n = (int64_t)max(1, (len + TK - 1) >> p.tile_shift) * units_per_seq;
+            if (begin < at + n) { s_b = b; s_start[0] = begin - at; break; }
+            at += n;
+        }
+    }
+    __syncthreads();
+    if (active) {
+        Cursor c;
+        c.b = s_b;
+        c.seat(p);
+        c.unit = static_cast<int>(s_start[0] / c.tiles);
+        c.tile = static_cast<int>(s_start[0] % c.tiles);
+        int64_t left = end - begin;
+        if (threadIdx.x == 0) {
+            p.desc[2 * blockIdx.x] = make_int4(c.b, c.unit, c.tile, c.tiles);
+            p.desc[2 * blockIdx.x + 1] = make_int4(ctas, 0, static_cast<int>(total & 0xffffffff), static_cast<int>(total >> 32));
+        }
+        if (warp == kDecWarps) {
+            // ---------------- producer ----------------
+            const int page_rows = 1 << p.page_shift, box_rows = min(page_rows, TK);
+            int n = 0;
+            bool ok = true;
+            for (; left > 0 && ok; --left, ++n) {
+                const int stage = n % kDecStages;
+                const int pos = c.tile * TK, valid = min(TK, c.len - pos), head = c.unit / p.chunks;
+                const int pages = valid > 0 ? (valid + box_rows - 1) / box_rows : 0;           // at most TK / 8 <= 32
+                int page = p.num_pages;
+                if (lane < pages) {
+                    page = p.page_table[(int64_t)c.b * p.max_pages + (pos >> p.page_shift) + lane];
+                    if (page < 0 || page >= p.num_pages) {
+                        page = p.num_pages;                        // out of the map's range: the copy fills in zeros
+                        if (p.err_flag) *p.err_flag = 1;
+                    }
+                }
+                if (n >= kDecStages) ok = mbar_wait(&s_empty[stage], static_cast<uint32_t>(n / kDecStages - 1) & 1u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&s_full[stage], pages * box_rows * ROWB * 2);
+                __syncwarp();
+                if (lane < pages) {
+                    const uint32_t kd = ring + stage * 2 * kTileBytes + lane * box_rows * CH, vd = kd + kTileBytes;
+                    const int row = pos & (page_rows - 1);
+#pragma unroll
+                    for (int ch = 0; ch < NCH; ++ch) tma_page_box(kd + ch * TK * CH, &kmap, ch * (D / NCH), row, head, page, &s_full[stage]);
+#pragma unroll
+                    for (int ch = 0; ch < NCH; ++ch) tma_page_box(vd + ch * TK * CH, &vmap, ch * (D / NCH), row, head, page, &s_full[stage]);
+                }
+                if (++c.tile == c.tiles) c.next_unit(p);
+            }
+            for (int s = max(0, n - kDecStages); s < n; ++s) mbar_wait(&s_full[s % kDecStages], static_cast<uint32_t>(s / kDecStages) & 1u);
+        } else {
+            // ---------------- consumers ----------------
+            const int g = lane >> 2, t4 = lane & 3;
+            bool ok = true;                                        // a wait that ran out: results void, control flow unchanged
+            int n = 0;
+            bool first_fragment = true;
+            while (left > 0) {
+                const int head = c.unit / p.chunks, q0 = (c.unit % p.chunks) * HPU, heads = min(HPU, p.group - q0);
+                // the query heads as B operand: column g of tile nt is head q0 + nt * 8 + g
+                uint32_t qf[NT][KS][2];
+                float fac[NT][2];                                  // score factor of this thread's two columns 2 t4, 2 t4 + 1
+                const float ks = p.scale_log2 * (p.k_scale ? __ldg(p.k_scale + head * p.scale_step) : 1.f);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const bool have = nt * 8 + g < heads;
+                    const __nv_bfloat16* qp = p.q + c.b * p.q_ss + (int64_t)(head * p.group + q0 + nt * 8 + (have ? g : 0)) * p.q_hs;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        if (E4M3) {                                // k order of the byte fragments: dims 4 t4 .. 4 t4 + 3 of each 16
+                            const uint2 v = have ? *reinterpret_cast<const uint2*>(qp + k * 16 + t4 * 4) : make_uint2(0, 0);
+                            qf[nt][k][0] = v.x;
+                            qf[nt][k][1] = v.y;
+                        } else {
+                            qf[nt][k][0] = have ? *reinterpret_cast<const uint32_t*>(qp + k * 16 + t4 * 2) : 0u;
+                            qf[nt][k][1] = have ? *reinterpret_cast<const uint32_t*>(qp + k * 16 + t4 * 2 + 8) : 0u;
+                        }
+                    }
+                    float up = 1.f;
+                    if (E4M3) {
+                        // f16 holds a bf16 exactly once its exponent fits: bring the head's largest entry to [2^14, 2^15)
+                        float mx = 0.f;
+#pragma unroll
+                        for (int k = 0; k < KS; ++k)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(qf[nt][k][e])), fabsf(bf16_hi(qf[nt][k][e]))));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        int e = 0;
+                        if (mx > 0.f && mx < INFINITY) e = max(static_cast<int>((__float_as_uint(mx) >> 23) & 0xff) - 127 - 14, -112);
+                        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                        up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+                        for (int k = 0; k < KS; ++k)
+#pragma unroll
+                            for (int w = 0; w < 2; ++w) qf[nt][k][w] = pack_f16x2(bf16_lo(qf[nt][k][w]) * down, bf16_hi(qf[nt][k][w]) * down);
+                    }
+                    fac[nt][0] = ks * __shfl_sync(0xffffffffu, up, t4 * 8);
+                    fac[nt][1] = ks * __shfl_sync(0xffffffffu, up, t4 * 8 + 4);
+                }
+                float o[NT][KS][4], m[NT][2], l[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[nt][k][e] = 0.f;
+                    m[nt][0] = m[nt][1] = -INFINITY;
+                    l[nt][0] = l[nt][1] = 0.f;
+                }
+                const int take = static_cast<int>(min((int64_t)(c.tiles - c.tile), left));
+                for (int i = 0; i < take; ++i, ++n) {
+                    const int stage = n % kDecStages;
+                    const int valid = c.len - (c.tile + i) * TK;
+                    ok = ok && mbar_wait(&s_full[stage], static_cast<uint32_t>(n / kDecStages) & 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok && warp * 16 < valid) {
+                        const uint32_t kt = ring + stage * 2 * kTileBytes, vt = kt + kTileBytes;
+                        auto at = [&](uint32_t tile, int row, int byte) {
+                            const int swz = CH == 128 ? (row & 7) << 4 : ((row >> 1) & 3) << 4;
+                            return tile + (byte / CH) * (TK * CH) + row * CH + ((byte % CH) ^ swz);
+                        };
+                        // ---- S^T = K Q^T ----
+                        float s[STEPS][NT][4];
+#pragma unroll
+                        for (int st = 0; st < STEPS; ++st) {
+                            const int r0 = (st * kDecWarps + warp) * 16;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[st][nt][e] = 0.f;
+                            if (r0 < valid) {
+                                if (E4M3) {
+#pragma unroll
+                                    for (int k2 = 0; k2 < KS / 2; ++k2) {
+                                        uint32_t a[4];
+                                        ldsm_x4(a, at(kt, r0 + (lane & 15), k2 * 32 + (lane >> 4) * 16));
+#pragma unroll
+                                        for (int hh = 0; hh < 2; ++hh) {
+                                            const uint32_t a0 = e4m3x2_to_f16x2(a[2 * hh]), a2 = e4m3x2_to_f16x2(a[2 * hh] >> 16);
+                                            const uint32_t a1 = e4m3x2_to_f16x2(a[2 * hh + 1]), a3 = e4m3x2_to_f16x2(a[2 * hh + 1] >> 16);
+#pragma unroll
+                                            for (int nt = 0; nt < NT; ++nt)
+                                                mma16816<true>(s[st][nt], a0, a1, a2, a3, qf[nt][2 * k2 + hh][0], qf[nt][2 * k2 + hh][1]);
+                                        }
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int k = 0; k < KS; ++k) {
+                                        uint32_t a[4];
+                                        ldsm_x4(a, at(kt, r0 + (lane & 15), k * 32 + (lane >> 4) * 16));
+#pragma unroll
+                                        for (int nt = 0; nt < NT; ++nt) mma16816<false>(s[st][nt], a[0], a[1], a[2], a[3], qf[nt][k][0], qf[nt][k][1]);
+                                    }
+                                }
+                            }
+                        }
+                        // ---- running softmax, one maximum per tile and head ----
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                            for (int st = 0; st < STEPS; ++st) {
+                                const int r = (st * kDecWarps + warp) * 16 + g;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float v = r + (e >> 1) * 8 < valid ? s[st][nt][e] * fac[nt][e & 1] : -INFINITY;
+                                    s[st][nt][e] = v;
+                                    top[e & 1] = fmaxf(top[e & 1], v);
+                                }
+                            }
+#pragma unroll
+                            for (int off = 4; off < 32; off <<= 1) {
+                                top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+                                top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+                            }
+                            const bool grown = top[0] > m[nt][0] || top[1] > m[nt][1];
+                            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float mn = fmaxf(m[nt][e], top[e]);
+                                    const float corr = mn == -INFINITY ? 1.f : ex2(m[nt][e] - mn);
+                                    m[nt][e] = mn;
+                                    l[nt][e] *= corr;
+#pragma unroll
+                                    for (int k = 0; k < KS; ++k) { o[nt][k][e] *= corr; o[nt][k][e + 2] *= corr; }
+                                }
+                            }
+#pragma unroll
+                            for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float mm = m[nt][e & 1];
+                                    const float pv = ex2(s[st][nt][e] - (mm == -INFINITY ? 0.f : mm));
+                                    s[st][nt][e] = pv;
+                                    l[nt][e & 1] += pv;
+                                }
+                        }
+                        // ---- O^T += V^T P^T ----
+#pragma unroll
+                        for (int st = 0; st < STEPS; ++st) {
+                            const int r0 = (st * kDecWarps + warp) * 16;
+                            if (r0 >= valid) break;                // warp-uniform
+                            if (r0 + 16 > valid) {
+                                // rows past the end hold whatever the page holds, and 0 x NaN is NaN: clear them
+                                const int rows = r0 + 16 - valid;
+                                for (int x = lane; x < rows * (CH / 16) * NCH; x += 32) {
+                                    const int r = valid + x / ((CH / 16) * NCH), y = x % ((CH / 16) * NCH);
+                                    const uint32_t a = vt + (y / (CH / 16)) * (TK * CH) + r * CH + (y % (CH / 16)) * 16;
+                                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0u) : "memory");
+                                }
+                                fence_proxy_async_smem();          // these stores before the copy that refills the stage
+                                __syncwarp();
+                            }
+                            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int hh = 0; hh < 2; ++hh) {   // positions 0-7, 8-15 of the group
+                                    const float x = s[st][nt][2 * hh], y = s[st][nt][2 * hh + 1];
+                                    if (E4M3) {
+                                        ph[nt][hh] = transpose8x8(pack_f16x2(x, y));
+                                    } else {
+                                        const uint32_t hi = pack_bf16x2(x, y);
+                                        ph[nt][hh] = transpose8x8(hi);
+                                        pl[nt][hh] = transpose8x8(pack_bf16x2(x - bf16_lo(hi), y - bf16_hi(hi)));
+                                    }
+                                }
+                            if (E4M3) {
+#pragma unroll
+                                for (int k2 = 0; k2 < KS / 2; ++k2) {
+                                    uint32_t a[4];
+                                    ldsm_x4_trans(a, at(vt, r0 + (lane & 15), k2 * 32 + (lane >> 4) * 16));
+#pragma unroll
+                                    for (int hh = 0; hh < 2; ++hh) {
+                                        // a word: two neighbouring dims of two positions -> one word per dim
+                                        const uint32_t e0 = e4m3x2_to_f16x2(a[2 * hh]), e1 = e4m3x2_to_f16x2(a[2 * hh] >> 16);
+                                        const uint32_t f0 = e4m3x2_to_f16x2(a[2 * hh + 1]), f1 = e4m3x2_to_f16x2(a[2 * hh + 1] >> 16);
+                                        const uint32_t a0 = __byte_perm(e0, e1, 0x5410), a1 = __byte_perm(e0, e1, 0x7632);
+                                        const uint32_t a2 = __byte_perm(f0, f1, 0x5410), a3 = __byte_perm(f0, f1, 0x7632);
+#pragma unroll
+                                        for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][2 * k2 + hh], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                                    }
+                                }
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < KS; ++k) {
+                                    uint32_t a[4];
+                                    ldsm_x4_trans(a, at(vt, r0 + (lane & 7) + ((lane >> 4) & 1) * 8, k * 32 + ((lane >> 3) & 1) * 16));
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt) {
+                                        mma16816<false>(o[nt][k], a[0], a[1], a[2], a[3], ph[nt][0], ph[nt][1]);
+                                        mma16816<false>(o[nt][k], a[0], a[1], a[2], a[3], pl[nt][0], pl[nt][1]);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_empty[stage]);
+                }
+                // ---- end of the piece: join the four warps ----
+                const bool whole = c.tile == 0 && take == c.tiles;
+                const int slot = first_fragment ? 0 : 1;           // a piece that starts with the CTA's range is piece 0
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+                        if (g == 0) {
+                            s_m[warp][nt * 8 + t4 * 2 + e] = m[nt][e];
+                            s_l[warp][nt * 8 + t4 * 2 + e] = l[nt][e];
+                        }
+                    }
+                consumer_barrier();
+                const float vs = p.v_scale ? __ldg(p.v_scale + head * p.scale_step) : 1.f;
+                float mine_w[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int h = nt * 8 + t4 * 2 + e;
+                        const float top = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
+                        mine_w[nt][e] = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - top);
+                    }
+                const size_t piece = ((size_t)blockIdx.x * 2 + slot) * HPU;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int half = 0; half < D / 64; ++half) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const int k = half * 4 + kk;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                // row g or g + 8 of the 16 dims: dims g, g + 8 in bf16, 2 g, 2 g + 1 from the byte pairs
+                                const int dim = kk * 16 + (E4M3 ? 2 * g + (e >> 1) : g + (e >> 1) * 8);
+                                merge[(warp * 8 + t4 * 2 + (e & 1)) * kMergeCols + dim] = o[nt][k][e] * mine_w[nt][e & 1];
+                            }
+                        }
+                        consumer_barrier();
+                        const int r = threadIdx.x >> 4, d4 = (threadIdx.x & 15) * 4, h = nt * 8 + r;
+                        if (h < heads) {
+                            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                            for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, s_m[w][h]);
+#pragma unroll
+                            for (int w = 0; w < kDecWarps; ++w) sum += s_m[w][h] == -INFINITY ? 0.f : s_l[w][h] * ex2(s_m[w][h] - top);
+                            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for (int w = 0; w < kDecWarps; ++w) {
+                                const float4 v = *reinterpret_cast<const float4*>(&merge[(w * 8 + r) * kMergeCols + d4]);
+                                acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+                            }
+                            const int d = half * 64 + d4;
+                            if (whole) {
+                                const float inv = sum == 0.f ? 0.f : vs / sum;
+                                uint2 w2;
+                                w2.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+                                w2.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+                                *reinterpret_cast<uint2*>(p.out + c.b * p.o_ss + (int64_t)(head * p.group + q0 + h) * p.o_hs + d) = w2;
+                            } else {
+                                acc.x *= vs; acc.y *= vs; acc.z *= vs; acc.w *= vs;
+                                *reinterpret_cast<float4*>(p.o + (piece + h) * D + d) = acc;
+                                if (d == 0) p.ml[piece + h] = make_float2(top, sum);
+                            }
+                        }
+                        consumer_barrier();
+                    }
+                left -= take;
+                c.tile += take;
+                first_fragment = false;
+                if (c.tile == c.tiles) c.next_unit(p);
+            }
+        }
+    }
+    pdl_trigger();
+}
+
+// Joins the pieces of the units that were cut.  CTA (c - 1, r) belongs to the cut between ranges c - 1 and c; it works if
+// that is the FIRST cut inside the unit there, and joins query head r of it: pieces c - 1 (its last), c, c + 1, ...
+constexpr int kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads)
+sdpa_decode_paged_join_kernel(const DecodeArgs p, int hpu) {
+    constexpr int SLICES = kJoinThreads / D;
+    __shared__ float s_w[kDecCtas], s_red[2][kJoinThreads / 32], s_acc[SLICES][D];
+    pdl_wait();
+    const int c = blockIdx.x + 1, r = blockIdx.y;
+    const int4 prev1 = p.desc[1], mine0 = p.desc[2 * c];
+    const int ctas = prev1.x;
+    const int64_t total = ((int64_t)prev1.w << 32) | (uint32_t)prev1.z;
+    if (c < ctas) {
+        const int64_t start = (int64_t)c * total / ctas, start_prev = (int64_t)(c - 1) * total / ctas;
+        const int f = mine0.z, tiles = mine0.w, b = mine0.x, unit = mine0.y;
+        const int head = unit / p.chunks, q0 = (unit % p.chunks) * hpu, heads = min(hpu, p.group - q0);
+        if (f > 0 && f <= start - start_prev && r < heads) {
+            const int64_t unit_end = start + (tiles - f);
+            const int last = static_cast<int>((unit_end * ctas + total - 1) / total) - 1;       // range that holds its last tile
+            const int n = last - (c - 1) + 1;
+            const int slot0 = f == start - start_prev ? 0 : 1;
+            auto piece = [&](int i) { return ((size_t)(c - 1 + i) * 2 + (i == 0 ? slot0 : 0)) * hpu + r; };
+            float top = -INFINITY;
+            for (int i = threadIdx.x; i < n; i += kJoinThreads) top = fmaxf(top, p.ml[piece(i)].x);
+            top = warp_max(top);
+            if ((threadIdx.x & 31) == 0) s_red[0][threadIdx.x >> 5] = top;
+            __syncthreads();
+            for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[0][w]);
+            float sum = 0.f;
+            for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+                const float2 ml = p.ml[piece(i)];
+                const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+                s_w[i] = w;
+                sum += w * ml.y;
+            }
+            sum = warp_sum(sum);
+            if ((threadIdx.x & 31) == 0) s_red[1][threadIdx.x >> 5] = sum;
+            __syncthreads();
+            sum = 0.f;
+            for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[1][w];
+            const int d = threadIdx.x % D, slice = threadIdx.x / D;
+            float acc = 0.f;
+#pragma unroll 8
+            for (int i = slice; i < n; i += SLICES) acc = fmaf(s_w[i], p.o[piece(i) * D + d], acc);
+            s_acc[slice][d] = acc;
+            __syncthreads();
+            if (slice == 0) {
+#pragma unroll
+                for (int s = 1; s < SLICES; ++s) acc += s_acc[s][d];
+                p.out[b * p.o_ss + (int64_t)(head * p.group + q0 + r) * p.o_hs + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+            }
+        }
+    }
+    pdl_trigger();
+}
+
+static int decode_nt(int64_t group) { return group > 8 ? 2 : 1; }
+
+template <int D, bool E4M3, int NT>
+static void launch_decode(const CUtensorMap& km, const CUtensorMap& vm, const DecodeArgs& p, int ctas, cudaStream_t st) {
+    auto kern = sdpa_decode_paged_kernel<D, E4M3, NT>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kDecSmem));
+    launch_kernel(kern, ctas, kDecThreads, kDecSmem, st, km, vm, p);
+    if (ctas > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(ctas - 1), static_cast<unsigned>(p.group < NT * 8 ? p.group : NT * 8));
+        cfg.blockDim = dim3(kJoinThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 1 : 0;
+        cudaLaunchKernelEx(&cfg, sdpa_decode_paged_join_kernel<D>, p, NT * 8);
+    }
+}
+
+}  // namespace nmt
+
+extern "C" {
+
+int64_t nmt_sdpa_decode_paged_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+    using namespace nmt;
+    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads) return 0;
+    const int64_t pieces = (int64_t)kDecCtas * 2 * decode_nt(heads / kv_heads) * 8;
+    return kDecCtas * 32 + pieces * (8 + 4 * head_dim);
+}
+
+int nmt_sdpa_decode_paged_bf16(const nmt_paged_cache* c, const void* q, int64_t q_ss, int64_t q_hs, void* out, int64_t o_ss, int64_t o_hs,
+                               int64_t heads, float scale, int32_t* err_flag, void* workspace, void* stream) {
+    using namespace nmt;
+    int st = check_paged_cache(c);
+    if (st != NMT_OK) return st;
+    if (heads <= 0 || heads % c->kv_heads || !(scale > 0.f) || !(scale < INFINITY)) return NMT_ERR_SHAPE;
+    const int64_t group = heads / c->kv_heads;
+    if (group > 65535) return NMT_ERR_UNSUPPORTED;
+    if (c->batch == 0) return NMT_OK;
+    if (!c->k || !c->v || !c->page_table || !c->seq_lens || !workspace) return NMT_ERR_NULL;
+    if ((st = check_view(q, c->batch, q_ss, heads, q_hs)) != NMT_OK || (st = check_view(out, c->batch, o_ss, heads, o_hs)) != NMT_OK) return st;
+    if (!aligned16(workspace) || !aligned4(err_flag)) return NMT_ERR_ALIGN;
+    EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return NMT_ERR_UNSUPPORTED;
+    const bool e4m3 = c->dtype == NMT_CACHE_E4M3;
+    const int64_t elt = e4m3 ? 1 : 2, row_bytes = c->head_dim * elt, tile = kTileBytes / row_bytes;
+    const int64_t chunk = row_bytes >= 128 ? 128 : 64;
+    CUtensorMap km, vm;
+    for (int i = 0; i < 2; ++i) {
+        const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->head_dim), static_cast<cuuint64_t>(c->page_size), static_cast<cuuint64_t>(c->kv_heads),
+                                    static_cast<cuuint64_t>(c->num_pages)};
+        const int64_t page = c->kv_heads * c->page_size * c->head_dim, ps = i ? c->v_page_stride : c->k_page_stride;
+        const cuuint64_t strides[3] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(c->page_size * row_bytes),
+                                       static_cast<cuuint64_t>((c->num_pages > 1 ? ps : page) * elt)};
+        const cuuint32_t box[4] = {static_cast<cuuint32_t>(chunk / elt), static_cast<cuuint32_t>(c->page_size < tile ? c->page_size : tile), 1, 1};
+        const cuuint32_t ones[4] = {1, 1, 1, 1};
+        if (encode(i ? &vm : &km, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? c->v : c->k, dims, strides, box, ones,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, chunk == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return NMT_ERR_UNSUPPORTED;
+    }
+    const int nt = decode_nt(group), hpu = nt * 8;
+    DecodeArgs p;
+    p.q = static_cast<const __nv_bfloat16*>(q); p.out = static_cast<__nv_bfloat16*>(out);
+    p.q_ss = q_ss; p.q_hs = q_hs; p.o_ss = o_ss; p.o_hs = o_hs;
+    p.seq_lens = c->seq_lens; p.page_table = c->page_table; p.k_scale = c->k_scale; p.v_scale = c->v_scale;
+    p.err_flag = err_flag;
+    p.desc = static_cast<int4*>(workspace);
+    p.ml = reinterpret_cast<float2*>(p.desc + 2 * kDecCtas);
+    p.o = reinterpret_cast<float*>(p.ml + (size_t)kDecCtas * 2 * hpu);
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.batch = static_cast<int>(c->batch); p.kv_heads = static_cast<int>(c->kv_heads); p.group = static_cast<int>(group);
+    p.chunks = static_cast<int>((group + hpu - 1) / hpu);
+    p.page_shift = log2_of(c->page_size); p.max_pages = static_cast<int>(c->max_pages); p.num_pages = static_cast<int>(c->num_pages);
+    p.scale_step = c->scale_count > 1 ? 1 : 0;
+    p.tile_shift = log2_of(tile);
+    // no more CTAs than there can be tiles
+    const int64_t cap = (c->max_pages * c->page_size + tile - 1) / tile, per_seq = cap * c->kv_heads * p.chunks;
+    const int ctas = per_seq >= kDecCtas || per_seq * c->batch >= kDecCtas ? kDecCtas : static_cast<int>(per_seq * c->batch);
+    cudaStream_t cs = static_cast<cudaStream_t>(stream);
+#define NMT_DEC_NT(D, E) do { if (nt == 2) launch_decode<D, E, 2>(km, vm, p, ctas, cs); else launch_decode<D, E, 1>(km, vm, p, ctas, cs); } while (0)
+    if (c->head_dim == 128) { if (e4m3) NMT_DEC_NT(128, true); else NMT_DEC_NT(128, false); }
+    else { if (e4m3) NMT_DEC_NT(64, true); else NMT_DEC_NT(64, false); }
+#undef NMT_DEC_NT
+    return finish_launch(ctas > 1 ? 2 : 1);
+}
+
+}  // extern "C"

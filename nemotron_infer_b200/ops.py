@@ -8,6 +8,8 @@ raises.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -248,6 +250,182 @@ def sdpa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
         raise ValueError("workspace too small")
     _lib.check(lib.nmt_sdpa_decode_bf16(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), k_new.data_ptr(),
                                         v_new.data_ptr(), int(s_cache), cap, H_Q, H_KV, D, workspace.data_ptr(), _stream()), "sdpa_decode")
+    return out
+
+
+def _on_device(fn):
+    """The operators over strided views and caches may be called with tensors of a device that is not the current one: they
+    run on that device, on its current stream."""
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        dev = first.device
+        if dev.type != "cuda":
+            raise ValueError("nemotron_infer_b200 operators run on CUDA tensors only (no CPU fallback)")
+        if dev.index == torch.cuda.current_device():
+            return fn(first, *args, **kwargs)
+        with torch.cuda.device(dev):
+            return fn(first, *args, **kwargs)
+    return call
+
+
+def _view3(t: torch.Tensor, name: str, rows: int | None, heads: int | None, dim: int, dev) -> tuple[int, int]:
+    """Checks a bf16 [rows, heads, dim] view (any row and head strides) and returns the two strides."""
+    shape = t.shape
+    if t.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != dim or (rows is not None and shape[0] != rows) or \
+            (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be bf16 [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {dim}], "
+                         f"got {t.dtype} {list(shape)}")
+    rs, hs, es = t.stride()
+    if es != 1 and dim > 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    if t.device != dev:
+        raise ValueError("all tensors must live on the same device")
+    return rs, hs
+
+
+def _result3(t: torch.Tensor, name: str, rows: int, heads: int, dim: int, dev) -> tuple[int, int]:
+    """The same for a tensor that is written: no two of its rows may share memory."""
+    rs, hs = _view3(t, name, rows, heads, dim, dev)
+    spans = sorted(((abs(s), n) for s, n in ((rs, rows), (hs, heads)) if n > 1))
+    need = dim
+    for s, n in spans:
+        if s < need:
+            raise ValueError(f"rows of {name} overlap in memory")
+        need = s * (n - 1) + need
+    return rs, hs
+
+
+def _i32(t: torch.Tensor, name: str, dev, shape: tuple[int, ...]) -> int:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)} on the caches' device")
+    return t.data_ptr()
+
+
+def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> "_lib.PagedCache":
+    """The C descriptor of a paged cache: k_cache / v_cache [num_pages, kv_heads, page_size, head_dim], bf16 or float8_e4m3fn,
+    each page contiguous; page_table int32 [batch, max_pages]; seq_lens int32 [batch]."""
+    dev, shape = k_cache.device, k_cache.shape
+    if k_cache.dtype is torch.bfloat16:
+        kind = 0
+    elif k_cache.dtype is torch.float8_e4m3fn:
+        kind = 1
+    else:
+        raise ValueError("the caches must be bf16 or float8_e4m3fn")
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype or v_cache.device != dev:
+        raise ValueError("k_cache and v_cache must both be [num_pages, kv_heads, page_size, head_dim] of one dtype on one device")
+    pages, heads, size, dim = shape
+    ks, vs = k_cache.stride(), v_cache.stride()
+    for st in (ks, vs):
+        if (dim > 1 and st[3] != 1) or (size > 1 and st[2] != dim) or (heads > 1 and st[1] != size * dim):
+            raise ValueError("every page of a cache must be contiguous [kv_heads, page_size, head_dim]")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be int32 [batch, max_pages]")
+    batch, max_pages = page_table.shape
+    count = 1
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is None:
+            continue
+        if t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous() or t.numel() not in (1, heads):
+            raise ValueError(f"{name} must be fp32 with 1 or kv_heads entries on the caches' device")
+        count = t.numel()
+    if k_scale is not None and v_scale is not None and k_scale.numel() != v_scale.numel():
+        raise ValueError("k_scale and v_scale must have the same number of entries")
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], vs[0], pages, size, heads, dim, kind,
+                           None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), count,
+                           _i32(page_table, "page_table", dev, (batch, max_pages)), _i32(seq_lens, "seq_lens", dev, (batch,)), batch, max_pages)
+
+
+def rope_table(positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """The rotation rows kv_append_paged reads: fp32 [positions, rot_dim], rot_dim / 2 cosines then as many sines of
+    position * base^(-2 i / rot_dim), angles in fp64 (a far position's angle is no longer exact in fp32)."""
+    inv = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    a = torch.arange(positions, dtype=torch.float64)[:, None] * inv
+    return torch.cat([a.cos(), a.sin()], dim=1).to(dtype=torch.float32).to(device)
+
+
+@_on_device
+def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    seq_lens: torch.Tensor, cu_new: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                    rope: torch.Tensor | None = None, interleaved: bool = False, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                    err_flag: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Writes the keys and values of new tokens, k / v [tokens, kv_heads, head_dim] bf16 (any strides), into the pages of
+    their sequences.  cu_new int32 [batch + 1]: the packed rows of each sequence, the last of which gets position
+    seq_lens[b] - 1 (seq_lens counts the new tokens already); rows behind cu_new[-1] are padding and left alone.  None:
+    one token per sequence.  With rope (fp32 [positions, rot_dim], see rope_table) K is rotated by position, and so is q
+    [tokens, q_heads, head_dim] when given: the result is q_out (q itself, for in place) or a new tensor, whose padding
+    rows are not written.  A float8_e4m3fn cache takes value / scale, saturated.  A token whose position, page or rope row
+    is out of range writes nothing and sets err_flag (device int32[1])."""
+    dev = k.device
+    c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale)
+    if k_cache.device != dev:
+        raise ValueError("all tensors must live on the same device")
+    if k.dim() != 3:
+        raise ValueError("k must be bf16 [tokens, kv_heads, head_dim]")
+    T = k.shape[0]
+    ks, vs = _view3(k, "k", T, c.kv_heads, c.head_dim, dev), _view3(v, "v", T, c.kv_heads, c.head_dim, dev)
+    cu = None if cu_new is None else _i32(cu_new, "cu_new", dev, (c.batch + 1,))
+    if cu is None and T != c.batch:
+        raise ValueError("without cu_new there is one token per sequence")
+    rows = rot = 0
+    if rope is not None:
+        if rope.dtype is not torch.float32 or rope.dim() != 2 or not rope.is_contiguous() or rope.device != dev:
+            raise ValueError("rope must be contiguous fp32 [positions, rot_dim] on the same device")
+        rows, rot = rope.shape
+    qs = os = (0, 0)
+    q_heads = 0
+    if q is not None:
+        if rope is None:
+            raise ValueError("q is only rotated: it needs rope")
+        qs = _view3(q, "q", T, None, c.head_dim, dev)
+        q_heads = q.shape[1]
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+        os = _result3(q_out, "q_out", T, q_heads, c.head_dim, dev)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _lib.check(_lib.load().nmt_kv_append_paged_bf16(
+        c, cu, T, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], None if rope is None else rope.data_ptr(), rows, rot,
+        1 if interleaved else 0, None if q is None else q.data_ptr(), qs[0], qs[1], q_heads, None if q is None else q_out.data_ptr(),
+        os[0], os[1], None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), _stream()), "kv_append_paged")
+    return q_out
+
+
+def sdpa_decode_paged_workspace(batch: int, heads: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Workspace of sdpa_decode_paged for these sizes; calls that may overlap on the GPU need one each."""
+    need = _lib.load().nmt_sdpa_decode_paged_workspace_bytes(batch, heads, kv_heads, head_dim)
+    return torch.empty(max(int(need), 16), dtype=torch.uint8, device=device)
+
+
+@_on_device
+def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                      scale: float | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                      err_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence, q [batch, heads, head_dim] bf16 (any strides), over the first seq_lens[b]
+    positions of its pages (the caches and tables kv_append_paged writes; append first, then the token sees itself).
+    scale defaults to 1 / sqrt(head_dim).  A sequence of length 0 gives zeros.  Page ids out of range read as zeros and set
+    err_flag (device int32[1]), as does a length past the page table."""
+    dev = q.device
+    c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale)
+    if k_cache.device != dev:
+        raise ValueError("all tensors must live on the same device")
+    if q.dim() != 3:
+        raise ValueError("q must be bf16 [batch, heads, head_dim]")
+    heads = q.shape[1]
+    qs = _view3(q, "q", c.batch, heads, c.head_dim, dev)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    os = _result3(out, "out", c.batch, heads, c.head_dim, dev)
+    lib = _lib.load()
+    if workspace is None:
+        workspace = sdpa_decode_paged_workspace(c.batch, heads, c.kv_heads, c.head_dim, dev)
+    elif workspace.device != dev or not workspace.is_contiguous() or \
+            workspace.numel() * workspace.element_size() < lib.nmt_sdpa_decode_paged_workspace_bytes(c.batch, heads, c.kv_heads, c.head_dim):
+        raise ValueError("workspace too small, not contiguous or on another device")
+    _lib.check(lib.nmt_sdpa_decode_paged_bf16(c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads,
+                                              c.head_dim ** -0.5 if scale is None else scale,
+                                              None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), workspace.data_ptr(),
+                                              _stream()), "sdpa_decode_paged")
     return out
 
 

@@ -1,0 +1,82 @@
+"""Inputs and plain 64-bit formulas for the tests of the paged cache and of prompt attention."""
+import math
+
+import torch
+
+BF = torch.bfloat16
+E4M3 = torch.float8_e4m3fn
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def pages_for(lens, page, g, spare=2, width=None):
+    """Scattered pages for the given lengths: (page table padded with ids out of range, number of pages)."""
+    need = [-(-n // page) for n in lens]
+    num = sum(need) + spare
+    perm = torch.randperm(num, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(lens), width or max(max(need), 1)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = perm[at:at + n]
+        at += n
+    return table, num
+
+
+def e4m3(x):
+    return x.clamp(-448, 448).to(E4M3)
+
+
+def rows_of(cache, table, b, n, scale=None):
+    """The first n cached rows of sequence b, [kv_heads, n, head_dim] in 64 bits; pages out of range are zeros."""
+    num, heads, page, dim = cache.shape
+    out = torch.zeros(heads, -(-n // page) * page, dim, dtype=torch.float64, device=cache.device)
+    for i, pg in enumerate(table[b, :-(-n // page)].tolist()):
+        if 0 <= pg < num:
+            out[:, i * page:(i + 1) * page] = cache[pg].double()
+    out = out[:, :n]
+    return out if scale is None else out * scale.double().reshape(-1, 1, 1)
+
+
+def attention64(q, k, v, sees, scale):
+    """q [n, H, D], k / v [G, m, D] in 64 bits, sees [n]: how many leading keys each query sees.  Returns the output and, for the
+    error bound, sum_j p_j |v_j| and the largest sum_d |q_d k_jd| * scale of a visible key, per query and head."""
+    n, H, D = q.shape
+    G, m = k.shape[0], k.shape[1]
+    qg = q.double().reshape(n, G, H // G, D).permute(1, 2, 0, 3)
+    if m == 0:
+        z = torch.zeros(n, H, D, dtype=torch.float64, device=q.device)
+        return z, z, z[..., :1]
+    vis = torch.arange(m, device=q.device)[None, :] < sees[:, None]
+    x = (qg @ k[:, None].transpose(-1, -2) * scale).masked_fill(~vis, -math.inf)
+    top = x.amax(-1, keepdim=True)
+    w = torch.exp(x - torch.where(top == -math.inf, torch.zeros_like(top), top))
+    w = torch.where(vis, w, torch.zeros_like(w))
+    w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
+    shape = lambda t: t.permute(2, 0, 1, 3).reshape(n, H, -1)
+    mag = (qg.abs() @ k[:, None].abs().transpose(-1, -2) * scale).masked_fill(~vis, 0).amax(-1, keepdim=True)
+    # a row of v that no query may see must not enter, whatever it holds
+    seen = vis.any(0)[None, :, None]
+    vv = torch.where(seen, v, torch.zeros_like(v))[:, None]
+    return shape(w @ vv), shape(w @ vv.abs()), shape(mag)
+
+
+def check(got, want, avg_abs, mag, weight_eps, terms, what):
+    """|got - want| against a derived bound.  got is rounded to bf16 once: half a step is 2^-8 of the value.  A weight is off by
+    a relative e = weight_eps (its own rounding before the product with v) + 2 * 2^-22 * (130 * mag + 4) (scores: products
+    of at most 128 elements accumulated in fp32 by the tensor core, at most one unit 2^-23 of the running sum's size per
+    step, the factor scale * log2 e, the subtraction of the maximum, all of size mag at most; 2^x good to 2^-22; twice,
+    once for the weight and once for the sum that divides it) + terms * 2^-22 (fp32 sums over the keys, in both).  The output then
+    moves by at most e * (sum_j p_j |v_j| + |out|), both at most 2 e sum_j p_j |v_j| together."""
+    e = weight_eps + 2 * 2.0 ** -22 * (130 * mag + 4) + terms * 2.0 ** -22
+    tol = 2.0 ** -8 * want.abs() + 2 * e * avg_abs * (1 + 2.0 ** -8) + 1e-30
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bool(bad.any()), (what, "elements off", int(bad.sum()), "worst", float((err / tol).nan_to_num(1e30).max()), bad.nonzero()[:4].tolist())

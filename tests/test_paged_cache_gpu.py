@@ -1,0 +1,330 @@
+"""kv_append_paged and sdpa_decode_paged against plain 64-bit formulas, at the sizes, layouts and contents where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+from paged_common import BF, E4M3, attention64, check, e4m3, gen, pages_for, randn, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(built_lib):
+    from nemotron_infer_b200 import ops as _ops
+    assert torch.cuda.is_available()
+    built_lib.nmt_set_device(torch.cuda.current_device())
+    yield _ops
+    torch.cuda.synchronize()
+    assert built_lib.nmt_device_wait_timeouts() == 0
+
+
+def make_caches(g, num, heads, page, dim, dtype, hole=None):
+    k, v = randn(g, num, heads, page, dim), randn(g, num, heads, page, dim)
+    if hole is not None:
+        k.fill_(hole)
+        v.fill_(hole)
+    return (e4m3(k * 50), e4m3(v * 50)) if dtype is E4M3 else (k.to(BF), v.to(BF))
+
+
+def rotate64(x, rows, interleaved):
+    x, r = x.double().clone(), rows.shape[1] // 2
+    c, s = rows[:, None, :r].double(), rows[:, None, r:].double()
+    a, b = (slice(0, 2 * r, 2), slice(1, 2 * r, 2)) if interleaved else (slice(0, r), slice(r, 2 * r))
+    xa, xb = x[..., a].clone(), x[..., b].clone()
+    x[..., a], x[..., b] = xa * c - xb * s, xb * c + xa * s
+    return x, (xa.abs() * c.abs() + xb.abs() * s.abs()).amax()
+
+
+def rounding(x, dtype):
+    """Half a step of the stored type at every value: relative 2^-8 in bf16, 2^-4 in e4m3 (2^-10 below its normal numbers)."""
+    return x.abs() * 2.0 ** -8 + 1e-38 if dtype is BF else torch.maximum(x.abs() * 2.0 ** -4, torch.full_like(x, 2.0 ** -10))
+
+
+@pytest.mark.parametrize("news,priors,page,heads,dim,q_heads,rot,interleaved,dtype,strided,pad", [
+    ([1, 1, 1], [0, 7, 63], 8, 8, 128, 40, 128, False, BF, False, 0),
+    ([1] * 33, list(range(33)), 16, 8, 128, 40, 0, False, E4M3, False, 0),
+    ([5, 0, 130, 1], [3, 9, 0, 500], 64, 2, 128, 10, 64, True, BF, True, 7),
+    ([257], [1], 32, 1, 64, 3, 16, False, BF, True, 0),
+    ([70, 1, 0], [0, 0, 0], 8, 3, 64, 6, 64, True, E4M3, True, 3),
+    ([64, 64], [0, 64], 1024, 4, 128, 4, 32, False, E4M3, False, 1),
+    ([0, 0], [4, 0], 16, 2, 64, 2, 64, False, BF, False, 5),
+])
+def test_append(ops, news, priors, page, heads, dim, q_heads, rot, interleaved, dtype, strided, pad):
+    g = gen(len(news) * 1000 + page)
+    lens = [n + p for n, p in zip(news, priors)]
+    T = sum(news)
+    table, num = pages_for(lens, page, g)
+    kc, vc = make_caches(g, num, heads, page, dim, dtype)
+    if strided:
+        x = randn(g, T + pad, q_heads + 2 * heads, dim).to(BF)
+        q, k, v = x[:, :q_heads], x[:, q_heads:q_heads + heads], x[:, q_heads + heads:]
+    else:
+        q, k, v = (randn(g, T + pad, h, dim).to(BF) for h in (q_heads, heads, heads))
+    rope = ops.rope_table(max(lens) + 3, rot) if rot else None
+    scales = (torch.rand(heads, generator=g, device="cuda") + 0.01, torch.rand(heads, generator=g, device="cuda") + 0.01) if dtype is E4M3 else (None, None)
+    one_each = all(n == 1 for n in news) and not pad
+    cu = None if one_each else torch.tensor([sum(news[:i]) for i in range(len(news) + 1)], dtype=torch.int32, device="cuda")
+    before = kc.clone(), vc.clone()
+    q_out = torch.full((T + pad, q_heads, dim), 7.0, dtype=BF, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    res = ops.kv_append_paged(k, v, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu, q=q if rot else None, rope=rope,
+                              interleaved=interleaved, k_scale=scales[0], v_scale=scales[1], q_out=q_out if rot else None, err_flag=err)
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    assert (res is q_out) if rot else (res is None)
+    want_k, want_v = before[0].double(), before[1].double()
+    touched = torch.zeros(num, heads, page, 1, dtype=torch.bool, device="cuda")
+    t = 0
+    for b, (n, p) in enumerate(zip(news, priors)):
+        for j in range(n):
+            pos = p + j
+            pg, at = int(table[b, pos // page]), pos % page
+            kr, qr = k[t:t + 1].double(), q[t:t + 1].double()
+            if rot:
+                kr, big = rotate64(k[t:t + 1], rope[pos:pos + 1], interleaved)
+                qr, big_q = rotate64(q[t:t + 1], rope[pos:pos + 1], interleaved)
+                # one fp32 product and one fused product-sum: two roundings of 2^-24 of the terms, then the stored type's
+                assert ((q_out[t:t + 1].double() - qr).abs() <= rounding(qr, BF) + 4 * 2.0 ** -24 * big_q).all()
+            want_k[pg, :, at] = kr[0] / (scales[0].double()[:, None] if scales[0] is not None else 1)
+            want_v[pg, :, at] = v[t].double() / (scales[1].double()[:, None] if scales[1] is not None else 1)
+            touched[pg, :, at] = True
+            t += 1
+    if dtype is E4M3:
+        want_k, want_v = want_k.clamp(-448, 448), want_v.clamp(-448, 448)
+    for got, want, old in ((kc, want_k, before[0]), (vc, want_v, before[1])):
+        # a value within an fp32 rounding of the border between two stored values may go to either: 2^-20 of slack
+        off = (got.double() - want).abs() > rounding(want, dtype) * (1 + 2.0 ** -12) + 2.0 ** -20
+        assert not bool((off & touched).any()), off.nonzero()[:4].tolist()
+        same = got.view(torch.uint8 if dtype is E4M3 else torch.int16) == old.view(torch.uint8 if dtype is E4M3 else torch.int16)
+        assert bool((same | touched).all()), "a row that is nobody's new token changed"
+    if rot and pad:
+        assert bool((q_out[T:] == 7.0).all()), "padding rows were written"
+
+
+def test_append_without_rotation_is_bit_exact_and_in_place_rotation_equals_out_of_place(ops):
+    g = gen(5)
+    lens = [100, 3]
+    table, num = pages_for(lens, 16, g)
+    cu = torch.tensor([0, 100, 103], dtype=torch.int32, device="cuda")
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    k, v, q = (randn(g, 103, h, 128).to(BF) for h in (2, 2, 10))
+    kc, vc = make_caches(g, num, 2, 16, 128, BF)
+    ops.kv_append_paged(k, v, kc, vc, table, sl, cu)
+    for b, (lo, n) in enumerate(((0, 100), (100, 3))):
+        assert torch.equal(rows_of(kc, table, b, n), k[lo:lo + n].double().transpose(0, 1))
+        assert torch.equal(rows_of(vc, table, b, n), v[lo:lo + n].double().transpose(0, 1))
+    rope = ops.rope_table(128, 128)
+    out = ops.kv_append_paged(k, v, kc, vc, table, sl, cu, q=q, rope=rope)
+    first = kc.clone()
+    q2 = q.clone()
+    assert ops.kv_append_paged(k, v, kc, vc, table, sl, cu, q=q2, rope=rope, q_out=q2) is q2
+    assert torch.equal(out, q2) and torch.equal(first, kc)
+
+
+def test_append_specials(ops):
+    """NaN stays NaN, what is past the type's range saturates, a zero stays a zero."""
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    kc, vc = (torch.zeros(1, 1, 8, 64, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    k = torch.zeros(1, 1, 64, dtype=BF, device="cuda")
+    k[0, 0, :5] = torch.tensor([math.nan, math.inf, -math.inf, 1e30, -500.0])
+    ops.kv_append_paged(k, k, kc, vc, table, torch.ones(1, dtype=torch.int32, device="cuda"))
+    got = kc[0, 0, 0].float()
+    assert math.isnan(got[0].item()) and got[1:5].tolist() == [448.0, -448.0, 448.0, -448.0] and not bool(got[5:].any())
+
+
+def test_append_out_of_range_writes_nothing_and_reports(ops):
+    g = gen(6)
+    k = randn(g, 4, 2, 64).to(BF)
+    rope = ops.rope_table(20, 64)
+    for lens, table, rows in (([0], [[0, 1]], 20), ([65], [[0, 1]], 80), ([4], [[9, 1]], 20), ([4], [[-1, 1]], 20), ([30], [[0, 1]], 20)):
+        kc, vc = make_caches(g, 2, 2, 32, 64, BF)
+        old = kc.clone(), vc.clone()
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        q = torch.full((4, 2, 64), 3.0, dtype=BF, device="cuda")
+        out = torch.full_like(q, 5.0)
+        ops.kv_append_paged(k, k, kc, vc, torch.tensor(table, dtype=torch.int32, device="cuda"), torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                            torch.tensor([0, 4], dtype=torch.int32, device="cuda"), q=q, rope=rope[:rows], q_out=out, err_flag=err)
+        assert err.item() == 1, lens
+        if lens != [65]:
+            assert torch.equal(kc, old[0]) and torch.equal(vc, old[1]) and bool((out == 5.0).all()), lens
+        else:                                                      # positions 61 .. 64 of 64: the first three have room, row 20.. of rope is missing
+            assert bool((out == 5.0).all()) and torch.equal(kc, old[0])
+
+
+DECODE = [
+    # lens, page, kv_heads, group, dim, dtype
+    ([512], 64, 8, 5, 128, BF),
+    ([1], 8, 8, 5, 128, BF),
+    ([0, 1, 63, 64, 65, 0, 127, 128, 129, 1000], 16, 8, 5, 128, BF),
+    ([0, 1, 63, 64, 65, 0, 127, 128, 129, 1000], 8, 2, 1, 64, BF),
+    ([300, 17, 4097], 32, 2, 16, 128, BF),
+    ([255, 256, 257, 3], 128, 1, 40, 64, BF),
+    ([40000], 64, 1, 8, 128, BF),
+    ([5, 70000, 1, 33], 256, 2, 4, 128, BF),
+    ([513, 2, 0, 4000], 16, 8, 5, 128, E4M3),
+    ([255, 256, 257, 1, 9], 8, 4, 3, 64, E4M3),
+    ([9000, 127, 128], 1024, 2, 12, 128, E4M3),
+    ([2049, 31], 64, 2, 9, 64, E4M3),
+    ([50] * 700, 16, 3, 7, 64, BF),
+]
+
+
+@pytest.mark.parametrize("lens,page,kv_heads,group,dim,dtype", DECODE)
+@pytest.mark.parametrize("peak", [1.0, 8.0])
+def test_decode(ops, lens, page, kv_heads, group, dim, dtype, peak):
+    g = gen(sum(lens) + page + group)
+    table, num = pages_for(lens, page, g)
+    kc, vc = make_caches(g, num, kv_heads, page, dim, dtype)
+    scales = (None, None)
+    if dtype is E4M3:
+        scales = tuple(0.01 * (1 + torch.rand(kv_heads, generator=g, device="cuda")) for _ in range(2))
+    # what lies behind a sequence's end in its last page must not matter
+    for b, n in enumerate(lens):
+        if n % page:
+            pg = int(table[b, n // page])
+            for c in (kc, vc):
+                c[pg, :, n % page:] = torch.full_like(c[pg, :, n % page:].float(), math.nan).to(c.dtype)
+    H = kv_heads * group
+    q = (peak * randn(g, len(lens), H, dim)).to(BF)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = ops.sdpa_decode_paged(q, kc, vc, table, sl, k_scale=scales[0], v_scale=scales[1], err_flag=err)
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    for b, n in enumerate(lens if len(lens) < 50 else lens[:20]):
+        k, v = rows_of(kc, table, b, n, scales[0]), rows_of(vc, table, b, n, scales[1])
+        want, avg, mag = attention64(q[b:b + 1], k, v, torch.tensor([n], device="cuda"), dim ** -0.5)
+        # weights: two bf16 terms, 2^-16; beside an e4m3 cache f16, 2^-11, and 2^-25 absolute below its normal numbers (n of them)
+        eps = 2.0 ** -16 if dtype is BF else 2.0 ** -11 + n * 2.0 ** -25
+        check(out[b:b + 1], want, avg, mag, eps, n, (b, n))
+    again = ops.sdpa_decode_paged(q, kc, vc, table, sl, k_scale=scales[0], v_scale=scales[1])
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16)), "the same call gave other bits"
+
+
+def test_decode_strides_scale_and_out(ops):
+    """q and out as views of wider tensors, K and V pages inside one allocation, an explicit scale."""
+    g = gen(11)
+    lens, page, G, dim = [77, 200, 5], 16, 2, 128
+    table, num = pages_for(lens, page, g)
+    both = randn(g, num, 2, G, page, dim).to(BF)
+    kc, vc = both[:, 0], both[:, 1]
+    wide = randn(g, 3, 3, 10, dim).to(BF)
+    out_wide = torch.full((10, 3, dim), 9.0, dtype=BF, device="cuda")
+    out = out_wide.transpose(0, 1)
+    q = wide[:, 1]
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    assert ops.sdpa_decode_paged(q, kc, vc, table, sl, scale=0.3, out=out) is out
+    for b, n in enumerate(lens):
+        want, avg, mag = attention64(q[b:b + 1], rows_of(kc, table, b, n), rows_of(vc, table, b, n), torch.tensor([n], device="cuda"), 0.3)
+        check(out[b:b + 1], want, avg, mag, 2.0 ** -16, n, b)
+    q2 = q.clone()
+    assert torch.equal(ops.sdpa_decode_paged(q2, kc, vc, table, sl, scale=0.3, out=q2), out)
+
+
+def test_decode_bad_pages_and_lengths(ops):
+    g = gen(12)
+    page, G, dim = 16, 2, 64
+    kc, vc = make_caches(g, 6, G, page, dim, BF)
+    table = torch.tensor([[0, 6, 1, 2], [3, 4, 5, -7]], dtype=torch.int32, device="cuda")
+    q = randn(g, 2, 4, dim).to(BF)
+    for lens, flag in (([60, 40], 1), ([10, 48], 0), ([10, 1 << 30], 1), ([16, 2147483647], 1), ([-5, 20], 0)):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = ops.sdpa_decode_paged(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), err_flag=err)
+        assert err.item() == flag, lens
+        for b, n in enumerate(lens):
+            n = min(max(n, 0), 64)
+            want, avg, mag = attention64(q[b:b + 1], rows_of(kc, table, b, n), rows_of(vc, table, b, n), torch.tensor([n], device="cuda"), dim ** -0.5)
+            check(out[b:b + 1], want, avg, mag, 2.0 ** -16, n, (lens, b))
+
+
+def test_decode_infinite_scores(ops):
+    """A score of -inf is a weight of zero; a whole row of them, or a NaN, is what the formula gives: nothing to average, NaN."""
+    page, dim = 8, 64
+    kc, vc = torch.zeros(2, 1, page, dim, dtype=BF, device="cuda"), torch.ones(2, 1, page, dim, dtype=BF, device="cuda")
+    kc[0, 0, 3, 0] = -math.inf
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, 1, dim, dtype=BF, device="cuda")
+    q[0, 0, 0] = 1.0
+    out = ops.sdpa_decode_paged(q, kc, vc, table, torch.tensor([12], dtype=torch.int32, device="cuda"))
+    assert bool((out == 1).all())
+    kc[0, 0, 3, 0] = math.nan
+    out = ops.sdpa_decode_paged(q, kc, vc, table, torch.tensor([12], dtype=torch.int32, device="cuda"))
+    assert bool(out.isnan().all())
+
+
+def test_decode_offsets_past_32_bits(ops):
+    """Pages far apart: element offsets past 2^32 in a cache of a few GB."""
+    page, G, dim = 64, 8, 128
+    num = 70000                                                    # 70000 * 64 KB * 2 bytes = 9 GB each
+    kc, vc = (torch.empty(num, G, page, dim, dtype=BF, device="cuda") for _ in range(2))
+    g = gen(13)
+    table = torch.tensor([[69999, 1, 69997], [40000, 65536, 2]], dtype=torch.int32, device="cuda")
+    for pg in table.flatten().tolist():
+        kc[pg], vc[pg] = randn(g, G, page, dim).to(BF), randn(g, G, page, dim).to(BF)
+    lens = [150, 192]
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    k, v = randn(g, 2, G, dim).to(BF), randn(g, 2, G, dim).to(BF)
+    ops.kv_append_paged(k, v, kc, vc, table, sl)
+    assert torch.equal(kc[69997, :, 149 - 128], k[0]) and torch.equal(vc[2, :, 63], v[1])
+    q = randn(g, 2, 40, dim).to(BF)
+    out = ops.sdpa_decode_paged(q, kc, vc, table, sl)
+    for b, n in enumerate(lens):
+        want, avg, mag = attention64(q[b:b + 1], rows_of(kc, table, b, n), rows_of(vc, table, b, n), torch.tensor([n], device="cuda"), dim ** -0.5)
+        check(out[b:b + 1], want, avg, mag, 2.0 ** -16, n, b)
+
+
+def test_steps_in_a_captured_graph_follow_the_lengths(ops):
+    """Append and attention captured once, replayed for growing sequences: the lengths live on the device."""
+    g = gen(14)
+    page, G, H, dim, B = 8, 2, 10, 128, 5
+    start = [0, 6, 7, 8, 100]
+    table, num = pages_for([n + 40 for n in start], page, g)
+    kc, vc = make_caches(g, num, G, page, dim, BF)
+    sl = torch.tensor(start, dtype=torch.int32, device="cuda")
+    x = torch.zeros(B, H + 2 * G, dim, dtype=BF, device="cuda")
+    rope = ops.rope_table(200, dim)
+    ws = ops.sdpa_decode_paged_workspace(B, H, G, dim)
+    q_out, out = torch.empty(B, H, dim, dtype=BF, device="cuda"), torch.empty(B, H, dim, dtype=BF, device="cuda")
+
+    def step():
+        sl.add_(1)
+        ops.kv_append_paged(x[:, H:H + G], x[:, H + G:], kc, vc, table, sl, q=x[:, :H], rope=rope, q_out=q_out)
+        ops.sdpa_decode_paged(q_out, kc, vc, table, sl, out=out, workspace=ws)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        sl.sub_(1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(30):
+        x.copy_(randn(g, B, H + 2 * G, dim))
+        graph.replay()
+        torch.cuda.synchronize()
+        if i % 6 == 5:
+            for b in range(B):
+                n = start[b] + i + 1
+                assert int(sl[b]) == n
+                want, avg, mag = attention64(q_out[b:b + 1], rows_of(kc, table, b, n), rows_of(vc, table, b, n), torch.tensor([n], device="cuda"), dim ** -0.5)
+                check(out[b:b + 1], want, avg, mag, 2.0 ** -16, n, (i, b))
+                kk, _ = rotate64(x[b:b + 1, H:H + G], rope[n - 1:n], False)
+                assert (rows_of(kc, table, b, n)[:, -1] - kk[0]).abs().max() <= kk.abs().max() * 2.0 ** -8 + 1e-5
+
+
+def test_other_stream(ops):
+    g = gen(15)
+    lens = [300]
+    table, num = pages_for(lens, 16, g)
+    kc, vc = make_caches(g, num, 2, 16, 128, BF)
+    q = randn(g, 1, 10, 128).to(BF)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = ops.sdpa_decode_paged(q, kc, vc, table, sl)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        out = ops.sdpa_decode_paged(q, kc, vc, table, sl)
+    side.synchronize()
+    assert torch.equal(out, want)
