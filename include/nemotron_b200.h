@@ -297,6 +297,26 @@ int nmt_sdpa_decode_paged_bf16(const nmt_paged_cache* cache, const void* q, int6
                                int64_t out_seq_stride, int64_t out_head_stride, int64_t heads, float scale, int32_t* err_flag,
                                void* workspace, void* stream);
 
+/* Attention of whole prompts, packed one after the other:
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, g]) v[j, g],   g = h / (heads / kv_heads),
+ * over the keys j of the query's own sequence; with causal != 0 query i of a sequence of n queries and m keys sees the keys
+ * j <= i + (m - n): the last query sees all of them, and a sequence whose first part is cached already passes more keys
+ * than queries.  A query that sees no key (m < n) gives zeros.  Stands where the reference calls sdpa_prefill_bf16
+ * (ops/attention/sdpa_prefill.cuh:332-395), with packed sequences and strides on top.
+ *   cu_q       device int32 [batch + 1], ascending: sequence b owns rows cu_q[b] .. cu_q[b + 1] - 1 of q and out.  Rows
+ *              behind cu_q[batch] are padding: out is not written there.  NULL (batch == 1): all rows.
+ *   cu_k       the same for k and v; NULL: cu_q when that is given, else all rows.
+ *   q, out bf16 [q_tokens][heads][head_dim], k, v bf16 [kv_tokens][kv_heads][head_dim], any token and head strides
+ *              (elements, multiples of 8): a view of a joint projection's output, or of the caches of
+ *              nmt_sdpa_decode_bf16.  head_dim 64 or 128, heads a multiple of kv_heads, scale positive and finite.
+ * fp32 scores, statistics and sums; the weights are rounded to bf16 once for the product with v.  What a mask hides is
+ * never used, not even an infinity or a NaN in v.  No workspace.  One launch. */
+int nmt_sdpa_prefill_bf16(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                          int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, void* out,
+                          int64_t out_token_stride, int64_t out_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch,
+                          int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                          void* stream);
+
 /* fp32 twin, unsplit; replaces causal_conv1d_prefill_fp32 (ops/mamba2/causal_conv1d.cuh:115-127). */
 int nmt_causal_conv1d_silu_f32(const float* x, const float* w, const float* bias, float* y, float* state_out,
                                int64_t conv_dim, int64_t S, int64_t batch, void* stream);

@@ -1,0 +1,598 @@
+// Attention of whole prompts on the 5th-generation tensor cores, causal or not, grouped heads, packed sequences.
+//
+//   out[i, h] = sum_j p_ij v[j, g],   p_ij = softmax_j(scale q[i, h] . k[j, g]),   j <= i + (m - n) when causal
+//
+// One pass over the keys with a running maximum M and sum L per query row:  P = 2^(c S - M),  L += sum P,  O += P V,
+// O *= 2^(M_old - M_new) when M moves (c = scale log2 e).  M is allowed to lag behind the true maximum by a factor of 2^8
+// - any M gives the same O / L - so after a row's first tiles O is hardly ever rescaled.
+//
+// A work item is 256 query rows of one head: two tiles of 128 rows that share every K / V tile of 128 keys.  One CTA per
+// SM, 16 warps with fixed roles:
+//   warps 0-3, 4-7   softmax of query tile 0 / 1: a thread owns a row.  Reads S from tensor memory, writes P (bf16) over it
+//   warps 8-11       epilogue: O / L -> bf16 -> global memory, while the other warps are at the next item already
+//   warp 12          issues the MMAs (one lane)
+//   warp 13          producer: tensor-map copies of Q, K, V into shared memory
+//   warp 14          scheduler: next item -> its sequence, rows and tile counts, published to everybody
+// S_t = Q_t K^T: tcgen05.mma 128 x 128 x 16 from shared memory (both operands rows of 128 bytes, 128-byte swizzle) into
+// tensor memory.  O_t += P_t V: A comes from tensor memory, where P_t lies over S_t's first 64 columns, B is V as it lies
+// in memory (keys x head_dim, so MN-major).  Columns 0-127 S_0 / P_0, 128-255 S_1 / P_1, 256-383 O_0, 384-511 O_1: all 512.
+// The MMAs of the two tiles alternate, PV_0 S_0' PV_1 S_1', so the tensor core works on one tile while the softmax warps are
+// on the other.  MMAs run in the order they are issued, and a commit covers all of them before it: "S_t is ready" also says
+// that the previous PV_t is done, which is what a rescale of O_t needs, so no other signal is exchanged per tile.
+#include "nmt_paged.cuh"
+#include "nmt_tensormap.cuh"
+#include "nmt_tma.cuh"
+
+namespace nmt {
+
+NMT_DEFINE_TIMEOUT_READER();
+
+constexpr int kPfThreads = 512;
+constexpr int kPfRows = 256;                                       // query rows of an item
+constexpr int kPfTile = 128;                                       // rows of a query tile, keys of a K / V tile
+constexpr int kSoftmaxRegs = 184, kEpilogueRegs = 64, kOtherRegs = 80;    // 2 x 184 + 64 + 80 = 512 = 4 x the launch's 128
+constexpr float kLag = 8.f;                                        // log2 of how far M may lag
+
+template <int D>
+struct PfShape {
+    static constexpr int kTileBytes = kPfTile * D * 2;             // Q tile, K tile or V tile
+    static constexpr int kStages = D == 128 ? 5 : 10;              // 160 KB of K / V tiles
+    static constexpr int kHalves = D / 64;                         // 64-column halves of 128-byte rows
+    static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
+};
+
+struct PrefillArgs {
+    __nv_bfloat16* out;
+    const __nv_bfloat16 *q, *k, *v;
+    const int32_t *cu_q, *cu_k;
+    int64_t o_ts, o_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+    float scale_log2;
+    int batch, q_tokens, kv_tokens, heads, group, causal, slots;
+};
+
+struct PfItem {
+    int q_row;       // first row of the item in q and out
+    int rows;        // valid rows, 1 .. 256
+    int kv_row;      // first key of the sequence in k and v
+    int kv_len;
+    int limit;       // keys that row 0 sees, before clamping; row r sees limit + r when causal
+    int head;
+    int n[2];        // K / V tiles of each query tile; n[0] < 0: no more items
+};
+
+// K-major operand in rows of 128 bytes, 128-byte swizzle: 1024 bytes between groups of 8 rows.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major operand in rows (k) of 128 bytes (64 n), 128-byte swizzle: 16 KB (a whole half) between blocks of 64 n, 1024 bytes
+// between groups of 8 k.
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1024ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// D fp32 (bits 4-5), A and B bf16 (bits 7-9, 10-12), B MN-major at bit 16, N / 8 at bits 17-22, M / 16 at bits 24-28.
+template <int N, bool B_MN>
+__host__ __device__ constexpr uint32_t idesc_bf16() {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (B_MN ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(kPfTile >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+#define NMT_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define NMT_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+// 32 columns of this warp's 32 lanes: thread = lane, register = column.
+__device__ __forceinline__ void tm_ld32(uint32_t* r, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+                 "%26,%27,%28,%29,%30,%31}, [%32];"
+                 : NMT_R8(r, 0), NMT_R8(r, 8), NMT_R8(r, 16), NMT_R8(r, 24) : "r"(addr));
+}
+__device__ __forceinline__ void tm_ld16(uint32_t* r, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : NMT_R8(r, 0), NMT_R8(r, 8) : "r"(addr));
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::NMT_W8(r, 0), NMT_W8(r, 8), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tma_rows(uint32_t smem_dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ float pf_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+struct PfBarriers {
+    uint64_t item_full[2], item_empty[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], l_full[2];
+    uint64_t kv_full[10], kv_empty[10];
+};
+
+// A lane-0 wait broadcast to the warp: everybody agrees on whether it ran out.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
+// Slot -> sequence and block of 256 rows.  Sequence b owns the slots from cu_q[b] / 256 + b on, at least one per block: no
+// prefix sum over the batch is needed, and at most one slot per sequence is empty.
+__device__ __forceinline__ bool decode_item(const PrefillArgs& p, int index, PfItem& it) {
+    const int lane = threadIdx.x & 31;
+    int slot = index / p.heads;
+    it.head = index % p.heads;
+    if (p.causal) slot = p.slots - 1 - slot;                       // the longest rows of a sequence first
+    int b = 0, q0 = 0, q1 = p.q_tokens, k0 = 0, k1 = p.kv_tokens;
+    if (p.cu_q) {
+        int lo = 0, len = p.batch;                                 // find_segment over the sequences' first slots
+        while (len > 0) {
+            const int step = (len + 31) >> 5, at = lane * step;
+            const bool ok = at < len && min(max(p.cu_q[lo + at], 0), p.q_tokens) / kPfRows + lo + at <= slot;
+            const int cnt = __popc(__ballot_sync(0xffffffffu, ok));
+            if (cnt == 0) break;
+            const int skip = (cnt - 1) * step + 1;
+            len = min(step - 1, len - skip);
+            lo += skip;
+        }
+        b = max(lo - 1, 0);
+        q0 = min(max(p.cu_q[b], 0), p.q_tokens);
+        q1 = min(max(p.cu_q[b + 1], q0), p.q_tokens);
+        const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
+        k0 = min(max(cu_k[b], 0), p.kv_tokens);
+        k1 = min(max(cu_k[b + 1], k0), p.kv_tokens);
+    }
+    const int block = slot - (q0 / kPfRows + b), n = q1 - q0, m = k1 - k0;
+    const int first = block * kPfRows;
+    if (block < 0 || first >= n) return false;
+    it.q_row = q0 + first;
+    it.rows = min(kPfRows, n - first);
+    it.kv_row = k0;
+    it.kv_len = m;
+    it.limit = p.causal ? first + 1 + (m - n) : m;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last = min(it.rows, (t + 1) * kPfTile) - 1;      // last valid row of the tile
+        const int sees = p.causal ? min(m, it.limit + last) : m;
+        it.n[t] = last < t * kPfTile ? 0 : max(1, (sees + kPfTile - 1) / kPfTile);
+    }
+    return true;
+}
+
+// One row again, by a warp on the CUDA cores, over the keys it sees and no others.  A tile product multiplies the hidden
+// keys' values by weights of zero, which is wrong where such a value is an infinity or a NaN (0 x NaN is NaN): the epilogue
+// sends a row here when its sum is finite and its output is not.  Without such values no call comes here.
+template <int D>
+__device__ __forceinline__ void redo_row(const PrefillArgs& p, const PfItem& it, int row, int sees, __nv_bfloat16* dst) {
+    constexpr int W = D / 64;                                      // words (pairs of elements) per lane
+    const int lane = threadIdx.x & 31;
+    const __nv_bfloat16* qp = p.q + (int64_t)(it.q_row + row) * p.q_ts + (int64_t)it.head * p.q_hs;
+    const __nv_bfloat16* kp = p.k + (int64_t)it.kv_row * p.k_ts + (int64_t)(it.head / p.group) * p.k_hs;
+    const __nv_bfloat16* vp = p.v + (int64_t)it.kv_row * p.v_ts + (int64_t)(it.head / p.group) * p.v_hs;
+    float2 q[W], o[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        q[i] = unpack2(*reinterpret_cast<const uint32_t*>(qp + i * 64 + lane * 2));
+        o[i] = make_float2(0.f, 0.f);
+    }
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < sees; ++j) {
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float2 k = unpack2(*reinterpret_cast<const uint32_t*>(kp + j * p.k_ts + i * 64 + lane * 2));
+            dot = fmaf(q[i].x, k.x, fmaf(q[i].y, k.y, dot));
+        }
+        const float s = warp_sum(dot) * p.scale_log2, to = fmaxf(m, s);
+        const float f = m == -INFINITY ? 0.f : exp2f(m - to), w = to == -INFINITY ? 0.f : exp2f(s - to);
+        const bool moved = to > m;                                 // a factor of one is left out: 0 x inf is no part of the formula
+        m = to;
+        l = (moved ? l * f : l) + w;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float2 v = unpack2(*reinterpret_cast<const uint32_t*>(vp + j * p.v_ts + i * 64 + lane * 2));
+            o[i].x = fmaf(w, v.x, moved ? o[i].x * f : o[i].x);
+            o[i].y = fmaf(w, v.y, moved ? o[i].y * f : o[i].y);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) *reinterpret_cast<uint32_t*>(dst + i * 64 + lane * 2) = pack_bf16x2(o[i].x / l, o[i].y / l);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPfThreads, 1)
+sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                    const PrefillArgs p) {
+    using Shape = PfShape<D>;
+    constexpr int ST = Shape::kStages;
+    extern __shared__ __align__(1024) uint8_t smem_p[];
+    __shared__ PfBarriers bar;
+    __shared__ PfItem s_item[2];
+    __shared__ float s_l[2][kPfTile];
+    __shared__ uint32_t s_tmem;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t q_smem = (smem_u32(smem_p) + 1023u) & ~1023u, ring = q_smem + 2 * Shape::kTileBytes;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.item_full[i], 1);
+            mbar_init(&bar.item_empty[i], 14);                     // warps 0-13
+            mbar_init(&bar.q_full[i], 1);
+            mbar_init(&bar.q_empty[i], 1);
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 4);
+            mbar_init(&bar.o_full[i], 1);
+            mbar_init(&bar.o_empty[i], 4);
+            mbar_init(&bar.l_full[i], 4);
+        }
+        for (int i = 0; i < ST; ++i) { mbar_init(&bar.kv_full[i], 1); mbar_init(&bar.kv_empty[i], 1); }
+        mbar_init_fence();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tm_fence_before();
+    __syncthreads();
+    tm_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
+    pdl_wait();
+
+    // Every role runs the same loop over the published items.  A wait that runs out (counted, nmt_tma.cuh) ends the role's
+    // loop; the other roles' waits then run out too, nothing is left waiting for good.
+    auto next_item = [&](int k, PfItem& it) {
+        if (!warp_wait(&bar.item_full[k & 1], static_cast<uint32_t>(k >> 1) & 1u)) return false;
+        it = s_item[k & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.item_empty[k & 1]);
+        return it.n[0] >= 0;
+    };
+
+    if (warp < 8) {
+        // ---------------- softmax ----------------
+        regs_up<kSoftmaxRegs>();
+        const int t = warp >> 2, wq = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + t * kPfTile, o_addr = tmem + lanes + 256 + t * kPfTile;
+        const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+        uint32_t s_uses = 0, o_uses = 0;
+        PfItem it;
+        for (int k = 0; next_item(k, it); ++k) {
+            const int tiles = t == 0 ? it.n[0] : it.n[1];
+            if (tiles == 0) continue;
+            const int row = t * kPfTile + wq * 32 + lane;
+            const int sees = p.causal ? min(it.kv_len, it.limit + row) : it.kv_len;
+            float m = -INFINITY;                                   // M / c
+            float2 l2 = make_float2(0.f, 0.f);
+            bool ok = true;
+            for (int j = 0; j < tiles; ++j) {
+                ok = warp_wait(&bar.s_full[t], s_uses & 1u);
+                if (!ok) break;
+                ++s_uses;
+                tm_fence_after();
+                float s[kPfTile];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tm_ld32(reinterpret_cast<uint32_t*>(s) + 32 * c, s_addr + 32 * c);
+                tm_wait_ld();
+                const int left = sees - j * kPfTile;
+                if (__any_sync(0xffffffffu, left < kPfTile)) {
+#pragma unroll
+                    for (int c = 0; c < kPfTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
+                }
+                float top = s[0];
+#pragma unroll
+                for (int c = 1; c < kPfTile; ++c) top = fmaxf(top, s[c]);
+                // M moves only when it has to: the first tile, or a maximum more than 2^8 above it
+                const bool move = (top - m) * p.scale_log2 > kLag || (m == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float to = move ? top : m;
+                    const float f = move ? pf_ex2((m - to) * p.scale_log2) : 1.f;       // m == -inf: 0
+                    l2.x *= f;
+                    l2.y *= f;
+                    if (j > 0) {
+                        uint32_t o[16];
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {          // rare, and 128 scores are live: few registers, no unrolling
+                            tm_ld16(o, o_addr + c);
+                            tm_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tm_st16(o_addr + c, o);
+                        }
+                    }
+                    m = to;
+                }
+                const float mc = m == -INFINITY ? 0.f : m * p.scale_log2;
+                const float2 nm2 = make_float2(-mc, -mc);
+                uint32_t pk[16];
+#pragma unroll
+                for (int c = 0; c < kPfTile; c += 32) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 x = __ffma2_rn(make_float2(s[c + e], s[c + e + 1]), c2, nm2);
+                        const float2 y = make_float2(pf_ex2(x.x), pf_ex2(x.y));
+                        l2 = __fadd2_rn(l2, y);
+                        pk[e / 2] = pack2(y);
+                    }
+                    tm_st16(s_addr + c / 2, pk);
+                }
+                tm_wait_st();
+                tm_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full[t]);
+            }
+            if (!ok) break;
+            if (o_uses > 0 && !warp_wait(&bar.o_empty[t], (o_uses - 1) & 1u)) break;    // the last item's L has been read
+            ++o_uses;
+            s_l[t][wq * 32 + lane] = l2.x + l2.y;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.l_full[t]);
+        }
+    } else if (warp < 12) {
+        // ---------------- epilogue ----------------
+        regs_down<kEpilogueRegs>();
+        const int wq = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+        uint32_t uses[2] = {0, 0};
+        PfItem it;
+        bool ok = true;
+        for (int k = 0; ok && next_item(k, it); ++k) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (it.n[t] == 0 || !ok) continue;
+                ok = warp_wait(&bar.l_full[t], uses[t] & 1u) && warp_wait(&bar.o_full[t], uses[t] & 1u);
+                if (!ok) continue;
+                ++uses[t];
+                tm_fence_after();
+                const int r = wq * 32 + lane, row = t * kPfTile + r;
+                const float l = s_l[t][r];
+                const int sees = p.causal ? min(it.kv_len, it.limit + row) : it.kv_len;
+                const float inv = 1.f / l;
+                __nv_bfloat16* dst = p.out + (int64_t)(it.q_row + row) * p.o_ts + (int64_t)it.head * p.o_hs;
+                bool odd = false;
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tm_ld32(o, tmem + lanes + 256 + t * kPfTile + c);
+                    tm_wait_ld();
+                    if (c + 32 == D) {                             // O and L are in registers: the next item may have them
+                        tm_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.o_empty[t]);
+                    }
+                    if (row < it.rows) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            float f[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                f[i] = sees > 0 && l != 0.f ? __uint_as_float(o[e + i]) * inv : 0.f;
+                                odd |= !(fabsf(f[i]) < INFINITY);
+                            }
+                            *reinterpret_cast<uint4*>(dst + c + e) = pack8(f);
+                        }
+                    }
+                }
+                for (uint32_t redo = __ballot_sync(0xffffffffu, odd && l < INFINITY); redo; redo &= redo - 1) {
+                    const int src = __ffs(redo) - 1, rr = t * kPfTile + wq * 32 + src;
+                    redo_row<D>(p, it, rr, p.causal ? min(it.kv_len, it.limit + rr) : it.kv_len,
+                                p.out + (int64_t)(it.q_row + rr) * p.o_ts + (int64_t)it.head * p.o_hs);
+                }
+            }
+        }
+    } else {
+        regs_down<kOtherRegs>();
+        if (warp == 12) {
+            // ---------------- MMA issuer ----------------
+            constexpr uint32_t kIdS = idesc_bf16<kPfTile, false>(), kIdO = idesc_bf16<D, true>();
+            uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, o_uses[2] = {0, 0}, kv = 0;      // kv: tiles taken from the ring
+            PfItem it;
+            bool ok = true;
+            auto stage_of = [&](uint32_t i) { return static_cast<int>(i % ST); };
+            auto wait_kv = [&](uint32_t i) { return warp_wait(&bar.kv_full[stage_of(i)], (i / ST) & 1u); };
+            auto scores = [&](int t, uint32_t ki) {                // S_t = Q_t K^T
+                if (lane == 0) {
+                    const uint32_t qa = q_smem + t * Shape::kTileBytes, ka = ring + stage_of(ki) * Shape::kTileBytes;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+                        mma_ss(tmem + t * kPfTile, desc_kmajor(qa + off), desc_kmajor(ka + off), kIdS, kk > 0);
+                    }
+                    mma_commit(&bar.s_full[t]);
+                }
+            };
+            for (int k = 0; ok && next_item(k, it); ++k) {
+                const int n_max = max(it.n[0], it.n[1]);
+                ok = wait_kv(kv);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (it.n[t] == 0 || !ok) continue;
+                    ok = warp_wait(&bar.q_full[t], q_uses[t]++ & 1u);
+                    if (!ok) continue;
+                    tm_fence_after();
+                    scores(t, kv);
+                    if (it.n[t] == 1 && lane == 0) mma_commit(&bar.q_empty[t]);
+                }
+                if (ok && lane == 0) mma_commit(&bar.kv_empty[stage_of(kv)]);
+                for (int j = 0; j < n_max && ok; ++j) {
+                    const uint32_t vi = kv + 2 * j + 1, ki = vi + 1;
+                    ok = wait_kv(vi);
+                    if (!ok) break;
+                    const uint32_t va = ring + stage_of(vi) * Shape::kTileBytes;
+                    const int valid = it.kv_len - j * kPfTile;
+                    if (valid < kPfTile) {
+                        // keys past the sequence's end belong to another one or to nobody, and 0 x NaN is NaN: clear their rows of V
+                        const int from = max(valid, 0);
+                        for (int x = lane; x < (kPfTile - from) * 8 * Shape::kHalves; x += 32) {
+                            const int r = from + x / (8 * Shape::kHalves), y = x % (8 * Shape::kHalves);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + (y >> 3) * 16384 + r * 128 + (y & 7) * 16), "r"(0u) : "memory");
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (!ok) continue;
+                        if (j < it.n[t]) {
+                            if (j == 0 && o_uses[t] > 0) ok = warp_wait(&bar.o_empty[t], (o_uses[t] - 1) & 1u);
+                            ok = ok && warp_wait(&bar.p_full[t], p_uses[t]++ & 1u);
+                            if (!ok) continue;
+                            tm_fence_after();
+                            if (lane == 0) {
+#pragma unroll
+                                for (int kk = 0; kk < kPfTile / 16; ++kk)
+                                    mma_ts(tmem + 256 + t * kPfTile, tmem + t * kPfTile + kk * 8, desc_mnmajor(va + kk * 2048), kIdO, j > 0 || kk > 0);
+                                if (j == it.n[t] - 1) mma_commit(&bar.o_full[t]);
+                            }
+                            if (j == it.n[t] - 1) ++o_uses[t];
+                        }
+                        if (j + 1 < n_max && t == 0) ok = wait_kv(ki);
+                        if (ok && j + 1 < it.n[t]) {
+                            tm_fence_after();
+                            scores(t, ki);
+                            if (j + 2 == it.n[t] && lane == 0) mma_commit(&bar.q_empty[t]);
+                        }
+                    }
+                    if (ok && lane == 0) {
+                        mma_commit(&bar.kv_empty[stage_of(vi)]);
+                        if (j + 1 < n_max) mma_commit(&bar.kv_empty[stage_of(ki)]);
+                    }
+                    __syncwarp();
+                }
+                kv += 2 * n_max;
+            }
+        } else if (warp == 13) {
+            // ---------------- producer ----------------
+            uint32_t q_uses[2] = {0, 0}, kv = 0;
+            PfItem it;
+            bool ok = true;
+            auto load = [&](const CUtensorMap* map, int head, int row, uint32_t dst, uint64_t* full) {
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(full, Shape::kTileBytes);
+#pragma unroll
+                    for (int h = 0; h < Shape::kHalves; ++h) tma_rows(dst + h * 16384, map, h * 64, head, row, full);
+                }
+            };
+            for (int k = 0; ok && next_item(k, it); ++k) {
+                const int n_max = max(it.n[0], it.n[1]), kv_head = it.head / p.group;
+                auto load_q = [&](int t) {
+                    if (it.n[t] == 0 || !ok) return;
+                    if (q_uses[t] > 0) ok = warp_wait(&bar.q_empty[t], (q_uses[t] - 1) & 1u);
+                    if (!ok) return;
+                    ++q_uses[t];
+                    load(&qmap, it.head, it.q_row + t * kPfTile, q_smem + t * Shape::kTileBytes, &bar.q_full[t]);
+                };
+                load_q(0);
+                for (int i = 0; i < 2 * n_max && ok; ++i, ++kv) {
+                    const int st = static_cast<int>(kv % ST);
+                    if (kv >= ST) ok = warp_wait(&bar.kv_empty[st], (kv / ST - 1) & 1u);
+                    if (!ok) break;
+                    load(i & 1 ? &vmap : &kmap, kv_head, it.kv_row + (i >> 1) * kPfTile, ring + st * Shape::kTileBytes, &bar.kv_full[st]);
+                    if (i == 0) load_q(1);
+                }
+            }
+            // no copy may still be under way when the CTA gives up its shared memory
+            if (lane == 0) {
+                for (uint32_t i = kv > ST ? kv - ST : 0; i < kv; ++i) mbar_wait(&bar.kv_full[i % ST], (i / ST) & 1u);
+                for (int t = 0; t < 2; ++t)
+                    if (q_uses[t] > 0) mbar_wait(&bar.q_full[t], (q_uses[t] - 1) & 1u);
+            }
+        } else if (warp == 14) {
+            // ---------------- scheduler ----------------
+            const int items = p.slots * p.heads;
+            int k = 0;
+            bool ok = true;
+            for (int index = blockIdx.x; ok; index += gridDim.x) {
+                PfItem it;
+                const bool more = index < items;
+                if (more && !decode_item(p, index, it)) continue;
+                if (k >= 2) ok = warp_wait(&bar.item_empty[k & 1], static_cast<uint32_t>((k >> 1) - 1) & 1u);
+                if (!ok) break;
+                if (!more) it.n[0] = -1;
+                if (lane == 0) {
+                    s_item[k & 1] = it;
+                    mbar_arrive(&bar.item_full[k & 1]);
+                }
+                ++k;
+                if (!more) break;
+            }
+        }
+    }
+    tm_fence_before();
+    __syncthreads();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    pdl_trigger();
+}
+
+template <int D>
+static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, cudaStream_t st) {
+    auto kern = sdpa_prefill_kernel<D>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PfShape<D>::kSmem));
+    const int64_t items = (int64_t)p.slots * p.heads;
+    launch_kernel(kern, static_cast<int>(items < kSmCount ? items : kSmCount), kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
+}
+
+}  // namespace nmt
+
+extern "C" {
+
+int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
+                          int64_t v_hs, void* out, int64_t o_ts, int64_t o_hs, const int32_t* cu_q, const int32_t* cu_k, int64_t batch,
+                          int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                          void* stream) {
+    using namespace nmt;
+    if (batch < 0 || q_tokens < 0 || kv_tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || !(scale > 0.f) || !(scale < INFINITY))
+        return NMT_ERR_SHAPE;
+    if ((!cu_q && (batch != 1 || cu_k))) return NMT_ERR_SHAPE;
+    if (head_dim != 64 && head_dim != 128) return NMT_ERR_UNSUPPORTED;
+    const int64_t slots = cu_q ? q_tokens / kPfRows + batch : (q_tokens + kPfRows - 1) / kPfRows;
+    if (q_tokens > 0x3fffffff || kv_tokens > 0x3fffffff || batch > 0x3fffffff || heads > 65535 || slots * heads > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
+    if (q_tokens == 0 || batch == 0) return NMT_OK;
+    int st;
+    if ((st = check_view(q, q_tokens, q_ts, heads, q_hs)) != NMT_OK || (st = check_view(out, q_tokens, o_ts, heads, o_hs)) != NMT_OK) return st;
+    if (kv_tokens > 0 && ((st = check_view(k, kv_tokens, k_ts, kv_heads, k_hs)) != NMT_OK || (st = check_view(v, kv_tokens, v_ts, kv_heads, v_hs)) != NMT_OK))
+        return st;
+    if (!aligned4(cu_q) || !aligned4(cu_k)) return NMT_ERR_ALIGN;
+    EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return NMT_ERR_UNSUPPORTED;
+    // Without keys there is nothing to describe (and nothing that is read counts): any valid row will do.
+    const bool none = kv_tokens == 0;
+    struct { const void* p; int64_t tokens, ts, heads, hs; } views[3] = {{q, q_tokens, q_ts, heads, q_hs},
+                                                                       {none ? q : k, none ? 1 : kv_tokens, k_ts, none ? 1 : kv_heads, k_hs},
+                                                                       {none ? q : v, none ? 1 : kv_tokens, v_ts, none ? 1 : kv_heads, v_hs}};
+    CUtensorMap maps[3];
+    for (int i = 0; i < 3; ++i) {
+        const auto& w = views[i];
+        const int64_t hs = w.heads > 1 ? w.hs : head_dim, ts = w.tokens > 1 ? w.ts : head_dim * w.heads;
+        if ((w.heads > 1 && hs < 1) || (w.tokens > 1 && ts < 1)) return NMT_ERR_UNSUPPORTED;       // a broadcast view
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(w.heads), static_cast<cuuint64_t>(w.tokens)};
+        const cuuint64_t strides[2] = {static_cast<cuuint64_t>(hs * 2), static_cast<cuuint64_t>(ts * 2)};
+        const cuuint32_t box[3] = {64, 1, kPfTile}, ones[3] = {1, 1, 1};
+        if (encode(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(w.p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return NMT_ERR_UNSUPPORTED;
+    }
+    PrefillArgs p;
+    p.out = static_cast<__nv_bfloat16*>(out);
+    p.q = static_cast<const __nv_bfloat16*>(q); p.k = static_cast<const __nv_bfloat16*>(k); p.v = static_cast<const __nv_bfloat16*>(v);
+    p.cu_q = cu_q; p.cu_k = cu_k; p.o_ts = o_ts; p.o_hs = o_hs;
+    p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.batch = static_cast<int>(batch); p.q_tokens = static_cast<int>(q_tokens); p.kv_tokens = static_cast<int>(kv_tokens);
+    p.heads = static_cast<int>(heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
+    p.slots = static_cast<int>(slots);
+    cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, cs); else launch_prefill<64>(maps[0], maps[1], maps[2], p, cs);
+    return finish_launch(1);
+}
+
+}  // extern "C"

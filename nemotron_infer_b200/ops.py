@@ -429,6 +429,43 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
+@_on_device
+def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                 cu_seqlens_k: torch.Tensor | None = None, causal: bool = True, scale: float | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of whole prompts, packed one after the other: q [tokens, heads, head_dim], k / v [kv_tokens, kv_heads,
+    head_dim], bf16 views with any token and head strides.  cu_seqlens int32 [batch + 1] (device) cuts the rows of q, and of
+    k and v unless cu_seqlens_k cuts those; None is one sequence of all rows.  With causal, query i of a sequence of n
+    queries and m keys sees keys j <= i + (m - n): a sequence whose first part is cached passes more keys than queries.  A
+    query that sees nothing gives zeros.  Rows behind the last sequence are not written.  scale defaults to
+    1 / sqrt(head_dim)."""
+    dev = q.device
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k and v must be bf16 [tokens, heads, head_dim]")
+    T, heads, dim = q.shape
+    T_k, kv_heads = k.shape[0], k.shape[1]
+    qs = _view3(q, "q", T, heads, dim, dev)
+    ks, vs = _view3(k, "k", T_k, kv_heads, dim, dev), _view3(v, "v", T_k, kv_heads, dim, dev)
+    batch, cu, cu_k = 1, None, None
+    if cu_seqlens is not None:
+        batch = cu_seqlens.numel() - 1
+        if batch < 0:
+            raise ValueError("cu_seqlens must have batch + 1 entries")
+        cu = _i32(cu_seqlens, "cu_seqlens", dev, (batch + 1,))
+        if cu_seqlens_k is not None:
+            cu_k = _i32(cu_seqlens_k, "cu_seqlens_k", dev, (batch + 1,))
+        elif T_k != T:
+            raise ValueError("with cu_seqlens alone, k and v have q's rows")
+    elif cu_seqlens_k is not None:
+        raise ValueError("cu_seqlens_k without cu_seqlens")
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    os = _result3(out, "out", T, heads, dim, dev)
+    _lib.check(_lib.load().nmt_sdpa_prefill_bf16(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                                 out.data_ptr(), os[0], os[1], cu, cu_k, batch, T, T_k, heads, kv_heads, dim,
+                                                 dim ** -0.5 if scale is None else scale, 1 if causal else 0, _stream()), "sdpa_prefill")
+    return out
+
+
 def ssm_decode_step(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: torch.Tensor,
                     state: torch.Tensor, dt_bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
                     dt_min: float = 0.0, dt_max: float = 3.4028234663852886e38) -> torch.Tensor:

@@ -125,3 +125,26 @@ def test_rope_table_is_exact_at_far_positions():
     for pos, i in ((200000, 0), (200000, 1), (131071, 5), (7, 31), (0, 3)):
         a = pos * 10000.0 ** (-2 * i / 64)
         assert abs(t[pos, i].item() - math.cos(a)) <= 2.0 ** -24 + 1e-9 and abs(t[pos, 32 + i].item() - math.sin(a)) <= 2.0 ** -24 + 1e-9
+
+
+def prefill(L, q=BUF, qts=5120, k=BUF, kts=1024, v=BUF, out=BUF, cu=BUF, cu_k=None, batch=2, T=5, T_k=5, heads=40, kv=8, dim=128, scale=0.1):
+    return L.nmt_sdpa_prefill_bf16(q, qts, 128, k, kts, 128, v, 1024, 128, out, 5120, 128, cu, cu_k, batch, T, T_k, heads, kv, dim, scale, 1, None)
+
+
+def test_prefill(built_lib):
+    L = built_lib
+    before = L.nmt_launch_count()
+    assert prefill(L, T=0) == OK and prefill(L, batch=0) == OK
+    assert prefill(L, T=-1) == SHAPE and prefill(L, T_k=-1) == SHAPE and prefill(L, batch=-1) == SHAPE
+    assert prefill(L, heads=12) == SHAPE and prefill(L, kv=0) == SHAPE
+    assert prefill(L, dim=96) == UNSUPPORTED
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        assert prefill(L, scale=scale) == SHAPE
+    assert prefill(L, cu=None) == SHAPE                            # one sequence, but batch 2
+    assert prefill(L, cu=None, cu_k=BUF, batch=1) == SHAPE
+    for name in ("q", "k", "v", "out"):
+        assert prefill(L, **{name: None}) == NULL and prefill(L, **{name: BUF + 8}) == ALIGN
+    assert prefill(L, qts=5124) == ALIGN and prefill(L, kts=-1024) == UNSUPPORTED
+    assert prefill(L, cu=BUF + 2) == ALIGN
+    assert prefill(L, T=1 << 31, T_k=1 << 31) == UNSUPPORTED
+    assert L.nmt_launch_count() == before

@@ -1,0 +1,193 @@
+"""sdpa_prefill against the plain 64-bit formula: lengths around the tile sizes, packed batches, head layouts, strides, empty rows."""
+import math
+
+import pytest
+import torch
+
+from paged_common import BF, attention64, check, gen, pages_for, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(built_lib):
+    from nemotron_infer_b200 import ops as _ops
+    assert torch.cuda.is_available()
+    built_lib.nmt_set_device(torch.cuda.current_device())
+    yield _ops
+    torch.cuda.synchronize()
+    assert built_lib.nmt_device_wait_timeouts() == 0
+
+
+def cu_of(lens):
+    return torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device="cuda")
+
+
+def compare(out, q, k, v, ns, ms, causal, scale, rows=None):
+    at = at_k = 0
+    for b, (n, m) in enumerate(zip(ns, ms)):
+        pick = torch.arange(n, device="cuda") if rows is None or n <= rows else torch.unique(torch.cat([torch.arange(40), torch.randint(0, n, (rows,)), torch.arange(n - 40, n)])).cuda()
+        sees = (pick + 1 + (m - n)).clamp(0, m) if causal else torch.full_like(pick, m)
+        kk, vv = k[at_k:at_k + m].double().transpose(0, 1), v[at_k:at_k + m].double().transpose(0, 1)
+        want, avg, mag = attention64(q[at:at + n][pick], kk, vv, sees, scale)
+        # the weights are rounded to bf16 for the product with v: 2^-8 each
+        check(out[at:at + n][pick], want, avg, mag, 2.0 ** -8, m, (b, n, m))
+        at, at_k = at + n, at_k + m
+
+
+CASES = [
+    # ns, ms (None: the same), heads, kv_heads, dim, causal
+    ([1], None, 5, 1, 128, True),
+    ([127], None, 4, 2, 128, True),
+    ([128], None, 2, 2, 128, True),
+    ([129], None, 10, 2, 128, True),
+    ([256], None, 2, 1, 64, True),
+    ([257], None, 3, 3, 64, True),
+    ([700], None, 10, 2, 128, False),
+    ([1500], None, 40, 8, 128, True),
+    ([1, 2, 3, 300, 0, 128, 255, 513, 0], None, 10, 2, 128, True),
+    ([1, 2, 3, 300, 0, 128, 255, 513, 0], None, 4, 4, 64, False),
+    ([100, 1, 300, 256], [1000, 700, 301, 256], 8, 2, 128, True),
+    ([100, 1, 300], [70, 900, 1024], 8, 1, 64, False),
+    ([300, 5, 200, 130], [100, 0, 199, 1], 4, 2, 128, True),          # fewer keys than queries: rows that see nothing
+    ([3], [0], 4, 2, 128, False),
+    ([4000], None, 2, 1, 128, True),
+    ([17] * 300, None, 5, 1, 64, True),
+]
+
+
+@pytest.mark.parametrize("ns,ms,heads,kv_heads,dim,causal", CASES)
+@pytest.mark.parametrize("peak", [1.0, 6.0])
+def test_against_the_formula(ops, ns, ms, heads, kv_heads, dim, causal, peak):
+    g = gen(sum(ns) + heads)
+    q = (peak * randn(g, sum(ns), heads, dim)).to(BF)
+    mm = ns if ms is None else ms
+    k, v = randn(g, sum(mm), kv_heads, dim).to(BF), randn(g, sum(mm), kv_heads, dim).to(BF)
+    out = ops.sdpa_prefill(q, k, v, cu_of(ns), None if ms is None else cu_of(ms), causal=causal)
+    torch.cuda.synchronize()
+    compare(out, q, k, v, ns if len(ns) < 50 else ns[:20], mm, causal, dim ** -0.5, rows=400)
+    again = ops.sdpa_prefill(q, k, v, cu_of(ns), None if ms is None else cu_of(ms), causal=causal)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16)), "the same call gave other bits"
+    if len(ns) == 1:
+        assert torch.equal(ops.sdpa_prefill(q, k, v, causal=causal).view(torch.int16), out.view(torch.int16))
+
+
+def test_long_prompt(ops):
+    g = gen(3)
+    n = 20011
+    q, k, v = randn(g, n, 2, 128).to(BF), randn(g, n, 1, 128).to(BF), randn(g, n, 1, 128).to(BF)
+    compare(ops.sdpa_prefill(q, k, v), q, k, v, [n], [n], True, 128 ** -0.5, rows=300)
+
+
+def test_growing_maximum(ops):
+    """Scores that climb along the keys: the running maximum moves at every tile, by more than the lag allows."""
+    n, dim = 1100, 128
+    g = gen(4)
+    q = torch.zeros(n, 2, dim, dtype=BF, device="cuda")
+    q[:, :, 0] = 16.0
+    k = 0.1 * randn(g, n, 1, dim)
+    k[:, 0, 0] = torch.arange(n, device="cuda") / 16
+    k, v = k.to(BF), randn(g, n, 1, dim).to(BF)
+    compare(ops.sdpa_prefill(q, k, v), q, k, v, [n], [n], True, dim ** -0.5)
+    k = k.flip(0).contiguous()
+    compare(ops.sdpa_prefill(q, k, v, causal=False), q, k, v, [n], [n], False, dim ** -0.5)
+
+
+def test_views_padding_and_out(ops):
+    """q, k, v as views of one projection's output, out transposed, padding rows untouched, an explicit scale."""
+    g = gen(7)
+    ns, pad, heads, kv, dim = [130, 77, 300], 50, 10, 2, 128
+    T = sum(ns)
+    x = randn(g, T + pad, heads + 2 * kv, dim).to(BF)
+    x[T:] = math.nan
+    q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    base = torch.full((heads, T + pad, dim), 3.0, dtype=BF, device="cuda")
+    out = base.transpose(0, 1)
+    assert ops.sdpa_prefill(q, k, v, cu_of(ns), scale=0.2, out=out) is out
+    compare(out, q, k, v, ns, ns, True, 0.2)
+    assert bool((out[T:] == 3.0).all()), "padding rows were written"
+
+
+def test_contiguous_cache_as_keys(ops):
+    """The caches of sdpa_decode, [kv_heads, capacity, 128], serve as keys and values: a chunk of 100 queries at 800 cached positions."""
+    g = gen(8)
+    kc, vc = randn(g, 8, 1024, 128).to(BF), randn(g, 8, 1024, 128).to(BF)
+    q = randn(g, 100, 40, 128).to(BF)
+    k, v = kc[:, :800].transpose(0, 1), vc[:, :800].transpose(0, 1)
+    compare(ops.sdpa_prefill(q, k, v), q, k, v, [100], [800], True, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_hidden_values_never_enter(ops, bad, dim):
+    """A non-finite key or value behind the mask, in the neighbouring sequence, or in the padding leaves a query's result alone."""
+    g = gen(9)
+    ns = [150, 90, 200]
+    q, k, v = randn(g, 440, 4, dim).to(BF), randn(g, 440, 2, dim).to(BF), randn(g, 440, 2, dim).to(BF)
+    clean = ops.sdpa_prefill(q, k, v, cu_of(ns))
+    k2, v2 = k.clone(), v.clone()
+    k2[150:240], v2[150:240] = bad, bad                            # the second sequence
+    hit = ops.sdpa_prefill(q, k2, v2, cu_of(ns))
+    assert torch.equal(hit[:150], clean[:150]) and torch.equal(hit[240:], clean[240:])
+    k3, v3 = k.clone(), v.clone()
+    k3[100, 1], v3[100, 1] = bad, bad                              # one key of the first: queries 0 .. 99 do not see it
+    hit = ops.sdpa_prefill(q, k3, v3, cu_of(ns))
+    compare(hit[:100], q, k, v, [100], [100], True, dim ** -0.5)
+    assert torch.equal(hit[150:], clean[150:]) and torch.equal(hit[:150, :2], clean[:150, :2])
+    v4 = v.clone()
+    v4[100, 1, 3] = bad                                            # values alone: the queries that see it get it, in that column
+    hit = ops.sdpa_prefill(q, k, v4, cu_of(ns))
+    compare(hit[:100], q, k, v, [100], [100], True, dim ** -0.5)
+    seen = hit[100:150, 2:, 3].float()
+    assert bool((seen.isnan() if math.isnan(bad) else seen == bad).all())
+    assert torch.equal(hit[100:150, 2:, 4:], clean[100:150, 2:, 4:]) or (hit[100:150, 2:, 4:].float() - clean[100:150, 2:, 4:].float()).abs().max() < 0.1
+
+
+def test_prompt_then_steps(ops):
+    """The operators as a server uses them: prompts appended to the pages and attended to, then single steps, against the whole
+    sequences at once."""
+    g = gen(10)
+    ns, steps, heads, kv, dim, page = [200, 37, 130], 6, 10, 2, 128, 16
+    B = len(ns)
+    total = [n + steps for n in ns]
+    table, num = pages_for(total, page, g)
+    kc, vc = (torch.zeros(num, kv, page, dim, dtype=BF, device="cuda") for _ in range(2))
+    rope = ops.rope_table(256, dim)
+    x = [randn(g, n, heads + 2 * kv, dim).to(BF) for n in total]   # every token's q | k | v, sequence by sequence
+    packed = torch.cat([t[:n] for t, n in zip(x, ns)])
+    lens = torch.tensor(ns, dtype=torch.int32, device="cuda")
+    q = ops.kv_append_paged(packed[:, heads:heads + kv], packed[:, heads + kv:], kc, vc, table, lens, cu_of(ns), q=packed[:, :heads], rope=rope)
+    # the rotated keys of the prompts, read back from the pages
+    rows = lambda c, b, n: torch.cat([c[int(p)] for p in table[b, :-(-n // page)]], dim=1)[:, :n].transpose(0, 1)
+    out = ops.sdpa_prefill(q, torch.cat([rows(kc, b, n) for b, n in enumerate(ns)]), packed[:, heads + kv:], cu_of(ns))
+    outs = [[o] for o in out.split(ns)]
+    qs = [[t] for t in q.split(ns)]
+    for i in range(steps):
+        lens += 1
+        one = torch.stack([t[n + i] for t, n in zip(x, ns)])
+        q1 = ops.kv_append_paged(one[:, heads:heads + kv], one[:, heads + kv:], kc, vc, table, lens, q=one[:, :heads], rope=rope)
+        o1 = ops.sdpa_decode_paged(q1, kc, vc, table, lens)
+        for b in range(B):
+            outs[b].append(o1[b:b + 1])
+            qs[b].append(q1[b:b + 1])
+    for b, n in enumerate(total):
+        compare(torch.cat(outs[b]), torch.cat(qs[b]), rows(kc, b, n), rows(vc, b, n), [n], [n], True, dim ** -0.5)
+
+
+def test_in_a_captured_graph(ops):
+    g = gen(12)
+    q, k, v = randn(g, 300, 4, 128).to(BF), randn(g, 300, 2, 128).to(BF), randn(g, 300, 2, 128).to(BF)
+    cu = cu_of([300, 0, 0])
+    out = torch.zeros_like(q)
+    ops.sdpa_prefill(q, k, v, cu, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.sdpa_prefill(q, k, v, cu, out=out)
+    for ns in ([100, 100, 100], [1, 299, 0], [0, 150, 10]):
+        out.fill_(5.0)
+        cu.copy_(cu_of(ns))
+        graph.replay()
+        torch.cuda.synchronize()
+        compare(out, q, k, v, ns, ns, True, 128 ** -0.5)
+        assert bool((out[sum(ns):] == 5.0).all())
