@@ -74,6 +74,33 @@ __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity) {
     return false;
 }
 
+// The same wait without a suspension hint: a waiter is woken as soon as the phase completes, which the hinted form above does
+// not promise (a ping-pong of waits of a few hundred cycles each ran at less than half its speed with it).  Bounded by the
+// clock: about two seconds, looked at every 256 polls.
+__device__ __forceinline__ bool mbar_try_wait_now(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_now(uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait_now(bar, parity)) return true;
+    uint64_t start, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait_now(bar, parity)) return true;
+        if ((i & 255u) == 0) {
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (now - start > 2000000000ull) break;
+        }
+    }
+    atomicAdd(&g_wait_timeouts, 1u);
+    return false;
+}
+
 // global -> shared bulk copy; completion (byte count) is signalled on `bar`.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"

@@ -11,8 +11,7 @@
 //   warps 0-3, 4-7   softmax of query tile 0 / 1: a thread owns a row.  Reads S from tensor memory, writes P (bf16) over it
 //   warps 8-11       epilogue: O / L -> bf16 -> global memory, while the other warps are at the next item already
 //   warp 12          issues the MMAs (one lane)
-//   warp 13          producer: tensor-map copies of Q, K, V into shared memory
-//   warp 14          scheduler: next item -> its sequence, rows and tile counts, published to everybody
+//   warp 13          producer: finds the next item, publishes it, and copies its Q, K, V into shared memory (tensor maps)
 // S_t = Q_t K^T: tcgen05.mma 128 x 128 x 16 from shared memory (both operands rows of 128 bytes, 128-byte swizzle) into
 // tensor memory.  O_t += P_t V: A comes from tensor memory, where P_t lies over S_t's first 64 columns, B is V as it lies
 // in memory (keys x head_dim, so MN-major).  Columns 0-127 S_0 / P_0, 128-255 S_1 / P_1, 256-383 O_0, 384-511 O_1: all 512.
@@ -30,7 +29,7 @@ NMT_DEFINE_TIMEOUT_READER();
 constexpr int kPfThreads = 512;
 constexpr int kPfRows = 256;                                       // query rows of an item
 constexpr int kPfTile = 128;                                       // rows of a query tile, keys of a K / V tile
-constexpr int kSoftmaxRegs = 184, kEpilogueRegs = 64, kOtherRegs = 80;    // 2 x 184 + 64 + 80 = 512 = 4 x the launch's 128
+constexpr int kSoftmaxRegs = 192, kEpilogueRegs = 64, kOtherRegs = 64;    // 2 x 192 + 64 + 64 = 512 = 4 x the launch's 128
 constexpr float kLag = 8.f;                                        // log2 of how far M may lag
 
 template <int D>
@@ -47,7 +46,7 @@ struct PrefillArgs {
     const int32_t *cu_q, *cu_k;
     int64_t o_ts, o_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
     float scale_log2;
-    int batch, q_tokens, kv_tokens, heads, group, causal, slots;
+    int batch, q_tokens, kv_tokens, heads, group, causal;
 };
 
 struct PfItem {
@@ -60,31 +59,38 @@ struct PfItem {
     int n[2];        // K / V tiles of each query tile; n[0] < 0: no more items
 };
 
-// K-major operand in rows of 128 bytes, 128-byte swizzle: 1024 bytes between groups of 8 rows.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-// MN-major operand in rows (k) of 128 bytes (64 n), 128-byte swizzle: 16 KB (a whole half) between blocks of 64 n, 1024 bytes
-// between groups of 8 k.
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1024ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
+// Shared-memory matrix descriptors, as two words so that a step along an operand is one 32-bit addition.  High word: 1024
+// bytes between groups of 8 rows (bits 32-45, in 16 bytes), version 1 (bit 46), 128-byte swizzle (2 at bit 61).  Low word:
+// address / 16, and at bit 16 the leading offset / 16.  K-major in rows of 128 bytes: not used, 1.  MN-major (V: rows are k,
+// 64 columns of n each): a whole half of the tile, 16 KB, to the next 64 columns.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mnmajor(uint32_t addr) { return (addr >> 4) | (1024u << 16); }
 // D fp32 (bits 4-5), A and B bf16 (bits 7-9, 10-12), B MN-major at bit 16, N / 8 at bits 17-22, M / 16 at bits 24-28.
 template <int N, bool B_MN>
 __host__ __device__ constexpr uint32_t idesc_bf16() {
     return (1u << 4) | (1u << 7) | (1u << 10) | (B_MN ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(kPfTile >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+    asm volatile("{ .reg .pred p; .reg .b64 da, db; setp.ne.b32 p, %4, 0; mov.b64 da, {%1, %5}; mov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p; }"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "r"(kDescHigh) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+    asm volatile("{ .reg .pred p; .reg .b64 db; setp.ne.b32 p, %4, 0; mov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p; }"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "r"(kDescHigh) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -114,58 +120,149 @@ __device__ __forceinline__ float pf_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The larger of three; a NaN among them is kept.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x on the FMA pipe, two at a time, for -inf < x < 128 (results below 2^-125 come out as 2^-125).  x = n + f with n the
+// nearest integer (adding 1.5 * 2^23 leaves it in the low bits of the sum), f in [-1/2, 1/2], and 2^f by a polynomial of
+// degree 4 with constant term 1, fitted for the least relative error (minimax, by linear programming): 2.9e-6 = 2^-18.4,
+// against the 2^-8 of the rounding to bf16 that follows.  n goes into the exponent by an integer addition.
+__device__ __forceinline__ float2 ex2_fma(const float2& x) {
+    const float2 magic = make_float2(12582912.f, 12582912.f);
+    const float2 xc = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+    const float2 t = __fadd2_rn(xc, magic);
+    const float2 f = __fadd2_rn(xc, __ffma2_rn(t, make_float2(-1.f, -1.f), magic));
+    float2 y = __ffma2_rn(f, make_float2(0.009582576341927052f, 0.009582576341927052f), make_float2(0.05590682849287987f, 0.05590682849287987f));
+    y = __ffma2_rn(y, f, make_float2(0.24024106562137604f, 0.24024106562137604f));
+    y = __ffma2_rn(y, f, make_float2(0.6931241154670715f, 0.6931241154670715f));
+    y = __ffma2_rn(y, f, make_float2(1.f, 1.f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
+// The weights of one row of a tile from its scores: w = 2^(s c - mc), added to the row sum in fp32, rounded to bf16 and
+// written over the scores in tensor memory, half a tile at a time so that the product with V can start on the first half.
+// PLAIN: every exponential on the special-function unit, exact zeros and NaN included (masked, infinite or NaN scores).
+// Otherwise kFmaPairs of every 8 pairs go to the FMA pipe: the special-function unit gives 16 results per cycle and SM,
+// which for 2 x 128 x 128 weights is as long as the four products that the tensor core does meanwhile.
+constexpr int kFmaPairs = 2;
+template <bool PLAIN>
+__device__ __forceinline__ void weights(const float (&s)[kPfTile], const float2& c2, float mc, float2& l2, uint32_t p_addr, int lane, uint64_t* half_bar,
+                                        uint64_t* full_bar) {
+    const float2 nm2 = make_float2(-mc, -mc);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * e], s[64 * h + 2 * e + 1]), c2, nm2);
+            const bool fma = !PLAIN && (e * kFmaPairs) % 8 < kFmaPairs;
+            const float2 y = fma ? ex2_fma(x) : make_float2(pf_ex2(x.x), pf_ex2(x.y));
+            sum[e & 1] = __fadd2_rn(sum[e & 1], y);
+            pk[e] = pack2(y);
+            if (e == 15) tm_st16(p_addr + 32 * h, pk);
+        }
+        tm_st16(p_addr + 32 * h + 16, pk + 16);
+        tm_wait_st();
+        tm_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(h == 0 ? half_bar : full_bar);
+    }
+    l2 = __fadd2_rn(l2, __fadd2_rn(sum[0], sum[1]));
+}
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 struct PfBarriers {
-    uint64_t item_full[2], item_empty[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], l_full[2];
-    uint64_t kv_full[10], kv_empty[10];
+    uint64_t item_full[2], item_empty[2], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], l_full[2];
+    uint64_t kv_full[10], kv_empty[10], taken;
 };
 
 // A lane-0 wait broadcast to the warp: everybody agrees on whether it ran out.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_now(bar, parity)); }
 
-// Slot -> sequence and block of 256 rows.  Sequence b owns the slots from cu_q[b] / 256 + b on, at least one per block: no
-// prefix sum over the batch is needed, and at most one slot per sequence is empty.
-__device__ __forceinline__ bool decode_item(const PrefillArgs& p, int index, PfItem& it) {
-    const int lane = threadIdx.x & 31;
-    int slot = index / p.heads;
-    it.head = index % p.heads;
-    if (p.causal) slot = p.slots - 1 - slot;                       // the longest rows of a sequence first
-    int b = 0, q0 = 0, q1 = p.q_tokens, k0 = 0, k1 = p.kv_tokens;
-    if (p.cu_q) {
-        int lo = 0, len = p.batch;                                 // find_segment over the sequences' first slots
-        while (len > 0) {
-            const int step = (len + 31) >> 5, at = lane * step;
-            const bool ok = at < len && min(max(p.cu_q[lo + at], 0), p.q_tokens) / kPfRows + lo + at <= slot;
-            const int cnt = __popc(__ballot_sync(0xffffffffu, ok));
-            if (cnt == 0) break;
-            const int skip = (cnt - 1) * step + 1;
-            len = min(step - 1, len - skip);
-            lo += skip;
+// Item number -> sequence, block of 256 rows, head.  Items go block index by block index from the highest down (over all
+// sequences that are long enough; heads fastest, so that the query heads of a kv head run side by side on its keys): when
+// causal, that is longest first, and the last items to start are the short ones.  The lengths are only known on the
+// device; a warp counts them as it goes - its numbers only ever grow, so it keeps its place.
+struct PfOrder {
+    int level, base, count, chunk, before;   // block index, items of higher blocks, sequences that have it; place among the sequences
+
+    __device__ __forceinline__ static int2 rows_of(const PrefillArgs& p, int b) {      // first row, rows
+        if (!p.cu_q) return make_int2(0, p.q_tokens);
+        const int q0 = min(max(p.cu_q[b], 0), p.q_tokens);
+        return make_int2(q0, min(max(p.cu_q[b + 1], q0), p.q_tokens) - q0);
+    }
+    __device__ __forceinline__ static bool has(const PrefillArgs& p, int b, int level) { return b < p.batch && rows_of(p, b).y > level * kPfRows; }
+    __device__ __forceinline__ void seat(const PrefillArgs& p, int lv) {
+        level = lv;
+        count = chunk = before = 0;
+        if (level < 0) return;
+        for (int b = threadIdx.x & 31; b - static_cast<int>(threadIdx.x & 31) < p.batch; b += 32) count += __popc(__ballot_sync(0xffffffffu, has(p, b, level)));
+    }
+    __device__ __forceinline__ void start(const PrefillArgs& p) {
+        int most = 0;
+        for (int b = threadIdx.x & 31; b < p.batch; b += 32) most = max(most, rows_of(p, b).y);
+        most = __reduce_max_sync(0xffffffffu, most);
+        base = 0;
+        seat(p, (most + kPfRows - 1) / kPfRows - 1);
+    }
+    // False: there is no such item.
+    __device__ __forceinline__ bool find(const PrefillArgs& p, int index, PfItem& it) {
+        const int lane = threadIdx.x & 31;
+        while (level >= 0 && index >= base + count * p.heads) {
+            base += count * p.heads;
+            seat(p, level - 1);
         }
-        b = max(lo - 1, 0);
-        q0 = min(max(p.cu_q[b], 0), p.q_tokens);
-        q1 = min(max(p.cu_q[b + 1], q0), p.q_tokens);
-        const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
-        k0 = min(max(cu_k[b], 0), p.kv_tokens);
-        k1 = min(max(cu_k[b + 1], k0), p.kv_tokens);
-    }
-    const int block = slot - (q0 / kPfRows + b), n = q1 - q0, m = k1 - k0;
-    const int first = block * kPfRows;
-    if (block < 0 || first >= n) return false;
-    it.q_row = q0 + first;
-    it.rows = min(kPfRows, n - first);
-    it.kv_row = k0;
-    it.kv_len = m;
-    it.limit = p.causal ? first + 1 + (m - n) : m;
+        if (level < 0) return false;
+        const int rank = (index - base) / p.heads;
+        it.head = (index - base) % p.heads;
+        uint32_t mask;
+        for (;;) {
+            mask = __ballot_sync(0xffffffffu, has(p, chunk + lane, level));
+            if (rank < before + __popc(mask) || chunk + 32 >= p.batch) break;
+            before += __popc(mask);
+            chunk += 32;
+        }
+        const bool pick = (mask >> lane & 1u) && __popc(mask & ((1u << lane) - 1u)) == rank - before;
+        const int b = min(chunk + max(__ffs(__ballot_sync(0xffffffffu, pick)) - 1, 0), p.batch - 1);
+        const int2 q = rows_of(p, b);
+        int k0 = 0, k1 = p.kv_tokens;
+        if (p.cu_q) {
+            const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
+            k0 = min(max(cu_k[b], 0), p.kv_tokens);
+            k1 = min(max(cu_k[b + 1], k0), p.kv_tokens);
+        }
+        const int first = level * kPfRows, n = q.y, m = k1 - k0;
+        it.q_row = q.x + first;
+        it.rows = min(kPfRows, n - first);
+        it.kv_row = k0;
+        it.kv_len = m;
+        it.limit = p.causal ? first + 1 + (m - n) : m;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int last = min(it.rows, (t + 1) * kPfTile) - 1;      // last valid row of the tile
-        const int sees = p.causal ? min(m, it.limit + last) : m;
-        it.n[t] = last < t * kPfTile ? 0 : max(1, (sees + kPfTile - 1) / kPfTile);
+        for (int t = 0; t < 2; ++t) {
+            const int last = min(it.rows, (t + 1) * kPfTile) - 1;  // last valid row of the tile
+            const int sees = p.causal ? min(m, it.limit + last) : m;
+            it.n[t] = last < t * kPfTile ? 0 : max(1, (sees + kPfTile - 1) / kPfTile);
+        }
+        return true;
     }
-    return true;
+};
+
+// The grid has a CTA for every item, but only one per SM fits: a running CTA takes over the work of one that has not started
+// yet (cluster launch control), so the items go to whoever is free.  The answer is 16 bytes in shared memory.
+__device__ __forceinline__ void ask_for_cta(void* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ int cta_taken(const void* answer) {     // its index, or -1: none was left
+    uint32_t ok, x;
+    asm volatile("{ .reg .pred p; .reg .b128 h; ld.shared.b128 h, [%2];\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h; selp.u32 %0, 1, 0, p; mov.u32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h; }"
+                 : "=r"(ok), "=r"(x) : "r"(smem_u32(answer)) : "memory");
+    return ok ? static_cast<int>(x) : -1;
 }
 
 // One row again, by a warp on the CUDA cores, over the keys it sees and no others.  A tile product multiplies the hidden
@@ -218,22 +315,25 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     extern __shared__ __align__(1024) uint8_t smem_p[];
     __shared__ PfBarriers bar;
     __shared__ PfItem s_item[2];
+    __shared__ __align__(16) uint4 s_answer;
     __shared__ float s_l[2][kPfTile];
     __shared__ uint32_t s_tmem;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = static_cast<int>(warp_uniform(threadIdx.x >> 5));
     const uint32_t q_smem = (smem_u32(smem_p) + 1023u) & ~1023u, ring = q_smem + 2 * Shape::kTileBytes;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.item_full[i], 1);
-            mbar_init(&bar.item_empty[i], 14);                     // warps 0-13
+            mbar_init(&bar.item_empty[i], 13);                     // warps 0-12
             mbar_init(&bar.q_full[i], 1);
             mbar_init(&bar.q_empty[i], 1);
             mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_half[i], 4);
             mbar_init(&bar.p_full[i], 4);
             mbar_init(&bar.o_full[i], 1);
             mbar_init(&bar.o_empty[i], 4);
             mbar_init(&bar.l_full[i], 4);
         }
+        mbar_init(&bar.taken, 1);
         for (int i = 0; i < ST; ++i) { mbar_init(&bar.kv_full[i], 1); mbar_init(&bar.kv_empty[i], 1); }
         mbar_init_fence();
     }
@@ -244,7 +344,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     tm_fence_before();
     __syncthreads();
     tm_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
+    const uint32_t tmem = warp_uniform(*reinterpret_cast<volatile uint32_t*>(&s_tmem));
     pdl_wait();
 
     // Every role runs the same loop over the published items.  A wait that runs out (counted, nmt_tma.cuh) ends the role's
@@ -280,17 +380,23 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 ++s_uses;
                 tm_fence_after();
                 float s[kPfTile];
+                float top4[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tm_ld32(reinterpret_cast<uint32_t*>(s) + 32 * c, s_addr + 32 * c);
                 tm_wait_ld();
                 const int left = sees - j * kPfTile;
-                if (__any_sync(0xffffffffu, left < kPfTile)) {
+                const bool masked = __any_sync(0xffffffffu, left < kPfTile);
+                if (masked) {
 #pragma unroll
                     for (int c = 0; c < kPfTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
                 }
-                float top = s[0];
 #pragma unroll
-                for (int c = 1; c < kPfTile; ++c) top = fmaxf(top, s[c]);
+                for (int c = 0; c < 4; ++c) {
+                    top4[c] = s[32 * c];
+#pragma unroll
+                    for (int e = 1; e < 31; e += 2) top4[c] = max3_nan(top4[c], s[32 * c + e], s[32 * c + e + 1]);
+                }
+                const float top = max3_nan(max3_nan(top4[0], s[31], s[63]), max3_nan(top4[1], s[95], s[127]), max3_nan(top4[2], top4[2], top4[3]));
                 // M moves only when it has to: the first tile, or a maximum more than 2^8 above it
                 const bool move = (top - m) * p.scale_log2 > kLag || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
@@ -312,23 +418,9 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     m = to;
                 }
                 const float mc = m == -INFINITY ? 0.f : m * p.scale_log2;
-                const float2 nm2 = make_float2(-mc, -mc);
-                uint32_t pk[16];
-#pragma unroll
-                for (int c = 0; c < kPfTile; c += 32) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 x = __ffma2_rn(make_float2(s[c + e], s[c + e + 1]), c2, nm2);
-                        const float2 y = make_float2(pf_ex2(x.x), pf_ex2(x.y));
-                        l2 = __fadd2_rn(l2, y);
-                        pk[e / 2] = pack2(y);
-                    }
-                    tm_st16(s_addr + c / 2, pk);
-                }
-                tm_wait_st();
-                tm_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[t]);
+                // a maximum that is not finite: a NaN or infinite score, or a row that sees nothing here
+                if (masked || __any_sync(0xffffffffu, !(fabsf(top) < INFINITY))) weights<true>(s, c2, mc, l2, s_addr, lane, &bar.p_half[t], &bar.p_full[t]);
+                else weights<false>(s, c2, mc, l2, s_addr, lane, &bar.p_half[t], &bar.p_full[t]);
             }
             if (!ok) break;
             if (o_uses > 0 && !warp_wait(&bar.o_empty[t], (o_uses - 1) & 1u)) break;    // the last item's L has been read
@@ -360,18 +452,18 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 __nv_bfloat16* dst = p.out + (int64_t)(it.q_row + row) * p.o_ts + (int64_t)it.head * p.o_hs;
                 bool odd = false;
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tm_ld32(o, tmem + lanes + 256 + t * kPfTile + c);
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t o[16];
+                    tm_ld16(o, tmem + lanes + 256 + t * kPfTile + c);
                     tm_wait_ld();
-                    if (c + 32 == D) {                             // O and L are in registers: the next item may have them
+                    if (c + 16 == D) {                             // O and L are in registers: the next item may have them
                         tm_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&bar.o_empty[t]);
                     }
                     if (row < it.rows) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
+                        for (int e = 0; e < 16; e += 8) {
                             float f[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
@@ -400,12 +492,13 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
             auto stage_of = [&](uint32_t i) { return static_cast<int>(i % ST); };
             auto wait_kv = [&](uint32_t i) { return warp_wait(&bar.kv_full[stage_of(i)], (i / ST) & 1u); };
             auto scores = [&](int t, uint32_t ki) {                // S_t = Q_t K^T
-                if (lane == 0) {
-                    const uint32_t qa = q_smem + t * Shape::kTileBytes, ka = ring + stage_of(ki) * Shape::kTileBytes;
+                const uint32_t qa = warp_uniform(desc_kmajor(q_smem + t * Shape::kTileBytes));
+                const uint32_t ka = warp_uniform(desc_kmajor(ring + stage_of(ki) * Shape::kTileBytes));
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                        mma_ss(tmem + t * kPfTile, desc_kmajor(qa + off), desc_kmajor(ka + off), kIdS, kk > 0);
+                        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4);
+                        mma_ss(tmem + t * kPfTile, qa + off, ka + off, kIdS, kk > 0);
                     }
                     mma_commit(&bar.s_full[t]);
                 }
@@ -420,14 +513,14 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     if (!ok) continue;
                     tm_fence_after();
                     scores(t, kv);
-                    if (it.n[t] == 1 && lane == 0) mma_commit(&bar.q_empty[t]);
+                    if (it.n[t] == 1 && elect_one()) mma_commit(&bar.q_empty[t]);
                 }
-                if (ok && lane == 0) mma_commit(&bar.kv_empty[stage_of(kv)]);
+                if (ok && elect_one()) mma_commit(&bar.kv_empty[stage_of(kv)]);
                 for (int j = 0; j < n_max && ok; ++j) {
                     const uint32_t vi = kv + 2 * j + 1, ki = vi + 1;
-                    ok = wait_kv(vi);
+                    ok = wait_kv(vi) && (j + 1 >= n_max || wait_kv(ki));
                     if (!ok) break;
-                    const uint32_t va = ring + stage_of(vi) * Shape::kTileBytes;
+                    const uint32_t va = ring + stage_of(vi) * Shape::kTileBytes, vd = warp_uniform(desc_mnmajor(va));
                     const int valid = it.kv_len - j * kPfTile;
                     if (valid < kPfTile) {
                         // keys past the sequence's end belong to another one or to nobody, and 0 x NaN is NaN: clear their rows of V
@@ -444,25 +537,29 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         if (!ok) continue;
                         if (j < it.n[t]) {
                             if (j == 0 && o_uses[t] > 0) ok = warp_wait(&bar.o_empty[t], (o_uses[t] - 1) & 1u);
-                            ok = ok && warp_wait(&bar.p_full[t], p_uses[t]++ & 1u);
-                            if (!ok) continue;
-                            tm_fence_after();
-                            if (lane == 0) {
+                            // the weights come in two halves of 64 keys
 #pragma unroll
-                                for (int kk = 0; kk < kPfTile / 16; ++kk)
-                                    mma_ts(tmem + 256 + t * kPfTile, tmem + t * kPfTile + kk * 8, desc_mnmajor(va + kk * 2048), kIdO, j > 0 || kk > 0);
-                                if (j == it.n[t] - 1) mma_commit(&bar.o_full[t]);
+                            for (int h = 0; h < 2; ++h) {
+                                ok = ok && warp_wait(h == 0 ? &bar.p_half[t] : &bar.p_full[t], p_uses[t] & 1u);
+                                if (!ok) continue;
+                                tm_fence_after();
+                                if (elect_one()) {
+#pragma unroll
+                                    for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                                        mma_ts(tmem + 256 + t * kPfTile, tmem + t * kPfTile + kk * 8, vd + kk * (2048 >> 4), kIdO, j > 0 || kk > 0);
+                                    if (h == 1 && j == it.n[t] - 1) mma_commit(&bar.o_full[t]);
+                                }
                             }
+                            ++p_uses[t];
+                            if (!ok) continue;
                             if (j == it.n[t] - 1) ++o_uses[t];
                         }
-                        if (j + 1 < n_max && t == 0) ok = wait_kv(ki);
-                        if (ok && j + 1 < it.n[t]) {
-                            tm_fence_after();
+                        if (j + 1 < it.n[t]) {
                             scores(t, ki);
-                            if (j + 2 == it.n[t] && lane == 0) mma_commit(&bar.q_empty[t]);
+                            if (j + 2 == it.n[t] && elect_one()) mma_commit(&bar.q_empty[t]);
                         }
                     }
-                    if (ok && lane == 0) {
+                    if (ok && elect_one()) {
                         mma_commit(&bar.kv_empty[stage_of(vi)]);
                         if (j + 1 < n_max) mma_commit(&bar.kv_empty[stage_of(ki)]);
                     }
@@ -473,16 +570,47 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         } else if (warp == 13) {
             // ---------------- producer ----------------
             uint32_t q_uses[2] = {0, 0}, kv = 0;
+            PfOrder order;
             PfItem it;
             bool ok = true;
             auto load = [&](const CUtensorMap* map, int head, int row, uint32_t dst, uint64_t* full) {
-                if (lane == 0) {
+                if (elect_one()) {
                     mbar_arrive_expect_tx(full, Shape::kTileBytes);
 #pragma unroll
                     for (int h = 0; h < Shape::kHalves; ++h) tma_rows(dst + h * 16384, map, h * 64, head, row, full);
                 }
             };
-            for (int k = 0; ok && next_item(k, it); ++k) {
+            auto publish = [&](int k) {
+                if (k >= 2) ok = warp_wait(&bar.item_empty[k & 1], static_cast<uint32_t>((k >> 1) - 1) & 1u);
+                if (ok && lane == 0) {
+                    s_item[k & 1] = it;
+                    mbar_arrive(&bar.item_full[k & 1]);
+                }
+                __syncwarp();
+            };
+            int k = 0, index = blockIdx.x, asked = 0;
+            order.start(p);
+            auto ask = [&] {
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&bar.taken, 16);
+                    ask_for_cta(&s_answer, &bar.taken);
+                }
+                ++asked;
+            };
+            auto answer = [&] {
+                if (!warp_wait(&bar.taken, static_cast<uint32_t>(asked - 1) & 1u)) return false;
+                index = cta_taken(&s_answer);
+                fence_proxy_async_smem();                          // this read before the next answer is written
+                __syncwarp();
+                return true;
+            };
+            while (ok && index >= 0) {
+                if (!order.find(p, index, it)) {                   // past the real number: take these CTAs out of the way too
+                    ask();
+                    ok = answer();
+                    continue;
+                }
+                publish(k++);
                 const int n_max = max(it.n[0], it.n[1]), kv_head = it.head / p.group;
                 auto load_q = [&](int t) {
                     if (it.n[t] == 0 || !ok) return;
@@ -491,39 +619,26 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     ++q_uses[t];
                     load(&qmap, it.head, it.q_row + t * kPfTile, q_smem + t * Shape::kTileBytes, &bar.q_full[t]);
                 };
-                load_q(0);
+                if (ok) load_q(0);
                 for (int i = 0; i < 2 * n_max && ok; ++i, ++kv) {
+                    // the next item is asked for when this one's last tiles go out, not earlier: whoever is free shall have it
+                    if (i == max(0, 2 * n_max - 4)) ask();
                     const int st = static_cast<int>(kv % ST);
                     if (kv >= ST) ok = warp_wait(&bar.kv_empty[st], (kv / ST - 1) & 1u);
                     if (!ok) break;
                     load(i & 1 ? &vmap : &kmap, kv_head, it.kv_row + (i >> 1) * kPfTile, ring + st * Shape::kTileBytes, &bar.kv_full[st]);
                     if (i == 0) load_q(1);
                 }
+                ok = ok && answer();
             }
+            it.n[0] = -1;
+            if (ok) publish(k);
             // no copy may still be under way when the CTA gives up its shared memory
             if (lane == 0) {
                 for (uint32_t i = kv > ST ? kv - ST : 0; i < kv; ++i) mbar_wait(&bar.kv_full[i % ST], (i / ST) & 1u);
                 for (int t = 0; t < 2; ++t)
                     if (q_uses[t] > 0) mbar_wait(&bar.q_full[t], (q_uses[t] - 1) & 1u);
-            }
-        } else if (warp == 14) {
-            // ---------------- scheduler ----------------
-            const int items = p.slots * p.heads;
-            int k = 0;
-            bool ok = true;
-            for (int index = blockIdx.x; ok; index += gridDim.x) {
-                PfItem it;
-                const bool more = index < items;
-                if (more && !decode_item(p, index, it)) continue;
-                if (k >= 2) ok = warp_wait(&bar.item_empty[k & 1], static_cast<uint32_t>((k >> 1) - 1) & 1u);
-                if (!ok) break;
-                if (!more) it.n[0] = -1;
-                if (lane == 0) {
-                    s_item[k & 1] = it;
-                    mbar_arrive(&bar.item_full[k & 1]);
-                }
-                ++k;
-                if (!more) break;
+                if (asked > 0) mbar_wait(&bar.taken, static_cast<uint32_t>(asked - 1) & 1u);
             }
         }
     }
@@ -534,11 +649,10 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
 }
 
 template <int D>
-static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, cudaStream_t st) {
+static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, int items, cudaStream_t st) {
     auto kern = sdpa_prefill_kernel<D>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PfShape<D>::kSmem));
-    const int64_t items = (int64_t)p.slots * p.heads;
-    launch_kernel(kern, static_cast<int>(items < kSmCount ? items : kSmCount), kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
+    launch_kernel(kern, items, kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
 }
 
 }  // namespace nmt
@@ -554,8 +668,10 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
         return NMT_ERR_SHAPE;
     if ((!cu_q && (batch != 1 || cu_k))) return NMT_ERR_SHAPE;
     if (head_dim != 64 && head_dim != 128) return NMT_ERR_UNSUPPORTED;
-    const int64_t slots = cu_q ? q_tokens / kPfRows + batch : (q_tokens + kPfRows - 1) / kPfRows;
-    if (q_tokens > 0x3fffffff || kv_tokens > 0x3fffffff || batch > 0x3fffffff || heads > 65535 || slots * heads > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
+    // Blocks of 256 rows: all that the batch can have (every sequence may end in a partly filled one); CTAs past the real
+    // number find nothing to do.
+    const int64_t full = (q_tokens + kPfRows - 1) / kPfRows, blocks = cu_q ? (q_tokens < full + batch - 1 ? q_tokens : full + batch - 1) : full;
+    if (q_tokens > 0x3fffffff || kv_tokens > 0x3fffffff || batch > 0x3fffffff || heads > 65535 || blocks * heads > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
     if (q_tokens == 0 || batch == 0) return NMT_OK;
     int st;
     if ((st = check_view(q, q_tokens, q_ts, heads, q_hs)) != NMT_OK || (st = check_view(out, q_tokens, o_ts, heads, o_hs)) != NMT_OK) return st;
@@ -589,9 +705,9 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
     p.scale_log2 = scale * 1.4426950408889634f;
     p.batch = static_cast<int>(batch); p.q_tokens = static_cast<int>(q_tokens); p.kv_tokens = static_cast<int>(kv_tokens);
     p.heads = static_cast<int>(heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
-    p.slots = static_cast<int>(slots);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, cs); else launch_prefill<64>(maps[0], maps[1], maps[2], p, cs);
+    const int items = static_cast<int>(blocks * heads);
+    if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, items, cs); else launch_prefill<64>(maps[0], maps[1], maps[2], p, items, cs);
     return finish_launch(1);
 }
 
