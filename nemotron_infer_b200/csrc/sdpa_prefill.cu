@@ -29,7 +29,7 @@ NMT_DEFINE_TIMEOUT_READER();
 constexpr int kPfThreads = 512;
 constexpr int kPfRows = 256;                                       // query rows of an item
 constexpr int kPfTile = 128;                                       // rows of a query tile, keys of a K / V tile
-constexpr int kSoftmaxRegs = 192, kEpilogueRegs = 64, kOtherRegs = 64;    // 2 x 192 + 64 + 64 = 512 = 4 x the launch's 128
+constexpr int kSoftmaxRegs = 200, kEpilogueRegs = 56, kOtherRegs = 56;    // 2 x 200 + 56 + 56 = 512 = 4 x the launch's 128
 constexpr float kLag = 8.f;                                        // log2 of how far M may lag
 
 template <int D>
@@ -46,7 +46,7 @@ struct PrefillArgs {
     const int32_t *cu_q, *cu_k;
     int64_t o_ts, o_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
     float scale_log2;
-    int batch, q_tokens, kv_tokens, heads, group, causal;
+    int batch, q_tokens, kv_tokens, heads, group, causal, out32;   // out32: rows of out are 32-byte aligned
 };
 
 struct PfItem {
@@ -177,7 +177,7 @@ template <int N> __device__ __forceinline__ void regs_down() { asm volatile("set
 
 struct PfBarriers {
     uint64_t item_full[2], item_empty[2], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], l_full[2];
-    uint64_t kv_full[10], kv_empty[10], taken;
+    uint64_t kv_full[10], kv_empty[10], v_raw, taken;
 };
 
 // A lane-0 wait broadcast to the warp: everybody agrees on whether it ran out.
@@ -333,6 +333,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
             mbar_init(&bar.o_empty[i], 4);
             mbar_init(&bar.l_full[i], 4);
         }
+        mbar_init(&bar.v_raw, 1);
         mbar_init(&bar.taken, 1);
         for (int i = 0; i < ST; ++i) { mbar_init(&bar.kv_full[i], 1); mbar_init(&bar.kv_empty[i], 1); }
         mbar_init_fence();
@@ -448,32 +449,40 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 const int r = wq * 32 + lane, row = t * kPfTile + r;
                 const float l = s_l[t][r];
                 const int sees = p.causal ? min(it.kv_len, it.limit + row) : it.kv_len;
-                const float inv = 1.f / l;
+                const bool none = sees <= 0 || l == 0.f;           // nothing to average: zeros, whatever the product holds
+                const float2 inv2 = make_float2(1.f / l, 1.f / l);
                 __nv_bfloat16* dst = p.out + (int64_t)(it.q_row + row) * p.o_ts + (int64_t)it.head * p.o_hs;
-                bool odd = false;
+                const uint32_t o_addr = tmem + lanes + 256 + t * kPfTile;
+                float2 odd2 = make_float2(0.f, 0.f);               // 0 x (a value that is not finite) is NaN
+                uint32_t o[2][16];
+                tm_ld16(o[0], o_addr);
 #pragma unroll
-                for (int c = 0; c < D; c += 16) {
-                    uint32_t o[16];
-                    tm_ld16(o, tmem + lanes + 256 + t * kPfTile + c);
+                for (int c = 0; c < D / 16; ++c) {
                     tm_wait_ld();
-                    if (c + 16 == D) {                             // O and L are in registers: the next item may have them
+                    if (c + 1 < D / 16) {
+                        tm_ld16(o[(c + 1) & 1], o_addr + 16 * (c + 1));
+                    } else {                                       // O and L are in registers: the next item may have them
                         tm_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&bar.o_empty[t]);
                     }
+                    uint32_t w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 f = __fmul2_rn(make_float2(__uint_as_float(o[c & 1][2 * e]), __uint_as_float(o[c & 1][2 * e + 1])), inv2);
+                        odd2 = __ffma2_rn(f, make_float2(0.f, 0.f), odd2);
+                        w[e] = none ? 0u : pack2(f);
+                    }
                     if (row < it.rows) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 8) {
-                            float f[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                f[i] = sees > 0 && l != 0.f ? __uint_as_float(o[e + i]) * inv : 0.f;
-                                odd |= !(fabsf(f[i]) < INFINITY);
-                            }
-                            *reinterpret_cast<uint4*>(dst + c + e) = pack8(f);
+                        if (p.out32) {
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 16 * c), NMT_W8(w, 0) : "memory");
+                        } else {
+                            *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(dst + 16 * c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
                         }
                     }
                 }
+                const bool odd = !none && row < it.rows && odd2.x + odd2.y != 0.f;
                 for (uint32_t redo = __ballot_sync(0xffffffffu, odd && l < INFINITY); redo; redo &= redo - 1) {
                     const int src = __ffs(redo) - 1, rr = t * kPfTile + wq * 32 + src;
                     redo_row<D>(p, it, rr, p.causal ? min(it.kv_len, it.limit + rr) : it.kv_len,
@@ -520,18 +529,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     const uint32_t vi = kv + 2 * j + 1, ki = vi + 1;
                     ok = wait_kv(vi) && (j + 1 >= n_max || wait_kv(ki));
                     if (!ok) break;
-                    const uint32_t va = ring + stage_of(vi) * Shape::kTileBytes, vd = warp_uniform(desc_mnmajor(va));
-                    const int valid = it.kv_len - j * kPfTile;
-                    if (valid < kPfTile) {
-                        // keys past the sequence's end belong to another one or to nobody, and 0 x NaN is NaN: clear their rows of V
-                        const int from = max(valid, 0);
-                        for (int x = lane; x < (kPfTile - from) * 8 * Shape::kHalves; x += 32) {
-                            const int r = from + x / (8 * Shape::kHalves), y = x % (8 * Shape::kHalves);
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + (y >> 3) * 16384 + r * 128 + (y & 7) * 16), "r"(0u) : "memory");
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
+                    const uint32_t vd = warp_uniform(desc_mnmajor(ring + stage_of(vi) * Shape::kTileBytes));
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (!ok) continue;
@@ -569,7 +567,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
             }
         } else if (warp == 13) {
             // ---------------- producer ----------------
-            uint32_t q_uses[2] = {0, 0}, kv = 0;
+            uint32_t q_uses[2] = {0, 0}, kv = 0, v_raws = 0;
             PfOrder order;
             PfItem it;
             bool ok = true;
@@ -626,7 +624,26 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     const int st = static_cast<int>(kv % ST);
                     if (kv >= ST) ok = warp_wait(&bar.kv_empty[st], (kv / ST - 1) & 1u);
                     if (!ok) break;
-                    load(i & 1 ? &vmap : &kmap, kv_head, it.kv_row + (i >> 1) * kPfTile, ring + st * Shape::kTileBytes, &bar.kv_full[st]);
+                    const uint32_t dst = ring + st * Shape::kTileBytes;
+                    const int valid = it.kv_len - (i >> 1) * kPfTile;
+                    if ((i & 1) && valid < kPfTile) {
+                        // Keys past the sequence's end belong to another one or to nobody, and 0 x NaN is NaN: their rows of V
+                        // are cleared before anybody is told that the tile is there.
+                        load(&vmap, kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.v_raw);
+                        ok = warp_wait(&bar.v_raw, v_raws++ & 1u);
+                        if (!ok) break;
+                        const int from = max(valid, 0);
+                        for (int x = lane; x < (kPfTile - from) * 8 * Shape::kHalves; x += 32) {
+                            const int r = from + x / (8 * Shape::kHalves), y = x % (8 * Shape::kHalves);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + (y >> 3) * 16384 + r * 128 + (y & 7) * 16), "r"(0u) : "memory");
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.kv_full[st]);
+                        __syncwarp();
+                    } else {
+                        load(i & 1 ? &vmap : &kmap, kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.kv_full[st]);
+                    }
                     if (i == 0) load_q(1);
                 }
                 ok = ok && answer();
@@ -638,6 +655,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 for (uint32_t i = kv > ST ? kv - ST : 0; i < kv; ++i) mbar_wait(&bar.kv_full[i % ST], (i / ST) & 1u);
                 for (int t = 0; t < 2; ++t)
                     if (q_uses[t] > 0) mbar_wait(&bar.q_full[t], (q_uses[t] - 1) & 1u);
+                if (v_raws > 0) mbar_wait(&bar.v_raw, (v_raws - 1) & 1u);
                 if (asked > 0) mbar_wait(&bar.taken, static_cast<uint32_t>(asked - 1) & 1u);
             }
         }
@@ -705,6 +723,7 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
     p.scale_log2 = scale * 1.4426950408889634f;
     p.batch = static_cast<int>(batch); p.q_tokens = static_cast<int>(q_tokens); p.kv_tokens = static_cast<int>(kv_tokens);
     p.heads = static_cast<int>(heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
+    p.out32 = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && (q_tokens == 1 || o_ts % 16 == 0) && (heads == 1 || o_hs % 16 == 0);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     const int items = static_cast<int>(blocks * heads);
     if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, items, cs); else launch_prefill<64>(maps[0], maps[1], maps[2], p, items, cs);
