@@ -6,8 +6,8 @@
 // O *= 2^(M_old - M_new) when M moves (c = scale log2 e).  M is allowed to lag behind the true maximum by a factor of 2^8
 // - any M gives the same O / L - so after a row's first tiles O is hardly ever rescaled.
 //
-// A work item is 256 query rows of one head: two tiles of 128 rows that share every K / V tile of 128 keys.  One CTA per
-// SM, 16 warps with fixed roles:
+// A work item is two query tiles, 128 rows of a head each, that share every K / V tile of 128 keys: two heads of a group on the
+// same rows, or the next rows (all of them, where there is one head per group).  One CTA per SM, 16 warps with fixed roles:
 //   warps 0-3, 4-7   softmax of query tile 0 / 1: a thread owns a row.  Reads S from tensor memory, writes P (bf16) over it
 //   warps 8-11       epilogue: O / L -> bf16 -> global memory, while the other warps are at the next item already
 //   warp 12          issues the MMAs (one lane)
@@ -27,7 +27,6 @@ namespace nmt {
 NMT_DEFINE_TIMEOUT_READER();
 
 constexpr int kPfThreads = 512;
-constexpr int kPfRows = 256;                                       // query rows of an item
 constexpr int kPfTile = 128;                                       // rows of a query tile, keys of a K / V tile
 constexpr int kSoftmaxRegs = 200, kEpilogueRegs = 56, kOtherRegs = 56;    // 2 x 200 + 56 + 56 = 512 = 4 x the launch's 128
 constexpr float kLag = 8.f;                                        // log2 of how far M may lag
@@ -46,17 +45,15 @@ struct PrefillArgs {
     const int32_t *cu_q, *cu_k;
     int64_t o_ts, o_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
     float scale_log2;
-    int batch, q_tokens, kv_tokens, heads, group, causal, out32;   // out32: rows of out are 32-byte aligned
+    int batch, q_tokens, kv_tokens, kv_heads, group, causal, out32;   // out32: rows of out are 32-byte aligned
 };
 
 struct PfItem {
-    int q_row;       // first row of the item in q and out
-    int rows;        // valid rows, 1 .. 256
-    int kv_row;      // first key of the sequence in k and v
-    int kv_len;
-    int limit;       // keys that row 0 sees, before clamping; row r sees limit + r when causal
-    int head;
-    int n[2];        // K / V tiles of each query tile; n[0] < 0: no more items
+    int kv_row;                                    // first key of the sequence in k and v
+    int kv_len, kv_head;
+    // per query tile: first row in q and out, valid rows (1 .. 128), keys that row 0 sees before clamping (row r sees limit + r
+    // when causal), head, K / V tiles.  n[0] < 0: no more items; n[1] == 0: one query tile only.  n[0] <= n[1] otherwise.
+    int q_row[2], rows[2], limit[2], head[2], n[2];
 };
 
 // Shared-memory matrix descriptors, as two words so that a step along an operand is one 32-bit addition.  High word: 1024
@@ -183,71 +180,105 @@ struct PfBarriers {
 // A lane-0 wait broadcast to the warp: everybody agrees on whether it ran out.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_now(bar, parity)); }
 
-// Item number -> sequence, block of 256 rows, head.  Items go block index by block index from the highest down (over all
-// sequences that are long enough; heads fastest, so that the query heads of a kv head run side by side on its keys): when
-// causal, that is longest first, and the last items to start are the short ones.  The lengths are only known on the
-// device; a warp counts them as it goes - its numbers only ever grow, so it keeps its place.
-struct PfOrder {
-    int level, base, count, chunk, before;   // block index, items of higher blocks, sequences that have it; place among the sequences
-
-    __device__ __forceinline__ static int2 rows_of(const PrefillArgs& p, int b) {      // first row, rows
-        if (!p.cu_q) return make_int2(0, p.q_tokens);
-        const int q0 = min(max(p.cu_q[b], 0), p.q_tokens);
-        return make_int2(q0, min(max(p.cu_q[b + 1], q0), p.q_tokens) - q0);
+// The query tiles of a sequence and kv head - blocks of 128 rows, and for each the heads of the group - are numbered block by
+// block, heads first, and an item is two neighbours: mostly two heads on the same rows, which see the same keys.  A short
+// prompt then fills both tiles of an item (with 256 rows of one head per item, 64 prompts of 128 tokens took 69 us instead of 55).
+// Items are handed out by their number of K / V tiles, most first, so that the last ones to start are short; among
+// equals sequence by sequence, kv heads fastest.  The lengths are only known on the device; a warp counts as it goes - the
+// numbers it is given only grow, so it keeps its place.
+struct PfSequence {
+    int q0, n, k0, m;                              // first query row, query rows, first key, keys
+    __device__ __forceinline__ PfSequence(const PrefillArgs& p, int b) : q0(0), n(p.q_tokens), k0(0), m(p.kv_tokens) {
+        if (!p.cu_q) return;
+        const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
+        q0 = min(max(p.cu_q[b], 0), p.q_tokens);
+        n = min(max(p.cu_q[b + 1], q0), p.q_tokens) - q0;
+        k0 = min(max(cu_k[b], 0), p.kv_tokens);
+        m = min(max(cu_k[b + 1], k0), p.kv_tokens) - k0;
     }
-    __device__ __forceinline__ static bool has(const PrefillArgs& p, int b, int level) { return b < p.batch && rows_of(p, b).y > level * kPfRows; }
-    __device__ __forceinline__ void seat(const PrefillArgs& p, int lv) {
-        level = lv;
-        count = chunk = before = 0;
-        if (level < 0) return;
-        for (int b = threadIdx.x & 31; b - static_cast<int>(threadIdx.x & 31) < p.batch; b += 32) count += __popc(__ballot_sync(0xffffffffu, has(p, b, level)));
+    __device__ __forceinline__ int tiles(const PrefillArgs& p) const { return (n + kPfTile - 1) / kPfTile * p.group; }
+    __device__ __forceinline__ int items(const PrefillArgs& p) const { return (tiles(p) + 1) / 2; }
+    // Items (the last ones) with at least `cost` K / V tiles; an item that sees nothing counts as one tile.
+    __device__ __forceinline__ int items_from(const PrefillArgs& p, int cost) const {
+        const int all = items(p), keys = (cost - 1) * kPfTile;     // such an item's last row sees more than `keys`
+        if (cost <= 1 || all == 0) return all;
+        if (m <= keys) return 0;
+        if (!p.causal) return all;
+        const int short_of = keys - (m - n);                       // the last row of block x sees m - n + min(n, 128 (x + 1)) keys
+        const int block = short_of < 0 ? 0 : min(short_of / kPfTile, (n - 1) / kPfTile);
+        return all - block * p.group / 2;                          // items whose second tile is in that block or a later one
+    }
+};
+struct PfOrder {
+    int cost, base, count, chunk, before;          // cost now handed out, items of higher cost, of this one; place among the sequences
+
+    __device__ __forceinline__ void seat(const PrefillArgs& p, int c) {
+        cost = c;
+        chunk = before = 0;
+        int mine = 0;
+        if (cost > 0)
+            for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
+                const PfSequence q(p, b);
+                mine += q.items_from(p, cost) - q.items_from(p, cost + 1);
+            }
+        count = __reduce_add_sync(0xffffffffu, mine);
     }
     __device__ __forceinline__ void start(const PrefillArgs& p) {
         int most = 0;
-        for (int b = threadIdx.x & 31; b < p.batch; b += 32) most = max(most, rows_of(p, b).y);
-        most = __reduce_max_sync(0xffffffffu, most);
+        for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
+            const PfSequence q(p, b);
+            if (q.n > 0) most = max(most, max(1, (q.m + kPfTile - 1) / kPfTile));
+        }
         base = 0;
-        seat(p, (most + kPfRows - 1) / kPfRows - 1);
+        seat(p, __reduce_max_sync(0xffffffffu, most));
     }
     // False: there is no such item.
     __device__ __forceinline__ bool find(const PrefillArgs& p, int index, PfItem& it) {
         const int lane = threadIdx.x & 31;
-        while (level >= 0 && index >= base + count * p.heads) {
-            base += count * p.heads;
-            seat(p, level - 1);
+        while (cost > 0 && index >= base + count * p.kv_heads) {
+            base += count * p.kv_heads;
+            seat(p, cost - 1);
         }
-        if (level < 0) return false;
-        const int rank = (index - base) / p.heads;
-        it.head = (index - base) % p.heads;
-        uint32_t mask;
+        if (cost <= 0) return false;
+        const int rank = (index - base) / p.kv_heads;
+        it.kv_head = (index - base) % p.kv_heads;
+        // the sequence whose share of this cost holds `rank`
+        int mine, upto;
         for (;;) {
-            mask = __ballot_sync(0xffffffffu, has(p, chunk + lane, level));
-            if (rank < before + __popc(mask) || chunk + 32 >= p.batch) break;
-            before += __popc(mask);
+            mine = 0;
+            if (chunk + lane < p.batch) {
+                const PfSequence q(p, chunk + lane);
+                mine = q.items_from(p, cost) - q.items_from(p, cost + 1);
+            }
+            upto = mine;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, upto, off);
+                if (lane >= off) upto += up;
+            }
+            const int sum = __shfl_sync(0xffffffffu, upto, 31);
+            if (rank < before + sum || chunk + 32 >= p.batch) break;
+            before += sum;
             chunk += 32;
         }
-        const bool pick = (mask >> lane & 1u) && __popc(mask & ((1u << lane) - 1u)) == rank - before;
-        const int b = min(chunk + max(__ffs(__ballot_sync(0xffffffffu, pick)) - 1, 0), p.batch - 1);
-        const int2 q = rows_of(p, b);
-        int k0 = 0, k1 = p.kv_tokens;
-        if (p.cu_q) {
-            const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
-            k0 = min(max(cu_k[b], 0), p.kv_tokens);
-            k1 = min(max(cu_k[b + 1], k0), p.kv_tokens);
-        }
-        const int first = level * kPfRows, n = q.y, m = k1 - k0;
-        it.q_row = q.x + first;
-        it.rows = min(kPfRows, n - first);
-        it.kv_row = k0;
-        it.kv_len = m;
-        it.limit = p.causal ? first + 1 + (m - n) : m;
+        const uint32_t holds = __ballot_sync(0xffffffffu, rank - before < upto && rank - before >= upto - mine);
+        const int src = max(__ffs(holds) - 1, 0);
+        const PfSequence q(p, min(chunk + src, p.batch - 1));
+        const int in_share = rank - before - __shfl_sync(0xffffffffu, upto - mine, src);
+        const int item = q.items(p) - q.items_from(p, cost) + in_share, tiles = q.tiles(p);
+        it.kv_row = q.k0;
+        it.kv_len = q.m;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int last = min(it.rows, (t + 1) * kPfTile) - 1;  // last valid row of the tile
-            const int sees = p.causal ? min(m, it.limit + last) : m;
-            it.n[t] = last < t * kPfTile ? 0 : max(1, (sees + kPfTile - 1) / kPfTile);
+            const int x = min(2 * item + t, tiles - 1), first = x / p.group * kPfTile;
+            it.head[t] = it.kv_head * p.group + x % p.group;
+            it.q_row[t] = q.q0 + first;
+            it.rows[t] = min(kPfTile, q.n - first);
+            it.limit[t] = p.causal ? first + 1 + (q.m - q.n) : q.m;
+            const int sees = p.causal ? min(q.m, it.limit[t] + it.rows[t] - 1) : q.m;
+            it.n[t] = 2 * item + t < tiles ? max(1, (sees + kPfTile - 1) / kPfTile) : 0;
         }
-        return true;
+        return holds != 0;
     }
 };
 
@@ -269,12 +300,13 @@ __device__ __forceinline__ int cta_taken(const void* answer) {     // its index,
 // keys' values by weights of zero, which is wrong where such a value is an infinity or a NaN (0 x NaN is NaN): the epilogue
 // sends a row here when its sum is finite and its output is not.  Without such values no call comes here.
 template <int D>
-__device__ __forceinline__ void redo_row(const PrefillArgs& p, const PfItem& it, int row, int sees, __nv_bfloat16* dst) {
+__device__ __forceinline__ void redo_row(const PrefillArgs& p, int q_row, int head, int kv_row, int sees) {
     constexpr int W = D / 64;                                      // words (pairs of elements) per lane
     const int lane = threadIdx.x & 31;
-    const __nv_bfloat16* qp = p.q + (int64_t)(it.q_row + row) * p.q_ts + (int64_t)it.head * p.q_hs;
-    const __nv_bfloat16* kp = p.k + (int64_t)it.kv_row * p.k_ts + (int64_t)(it.head / p.group) * p.k_hs;
-    const __nv_bfloat16* vp = p.v + (int64_t)it.kv_row * p.v_ts + (int64_t)(it.head / p.group) * p.v_hs;
+    const __nv_bfloat16* qp = p.q + (int64_t)q_row * p.q_ts + (int64_t)head * p.q_hs;
+    const __nv_bfloat16* kp = p.k + (int64_t)kv_row * p.k_ts + (int64_t)(head / p.group) * p.k_hs;
+    const __nv_bfloat16* vp = p.v + (int64_t)kv_row * p.v_ts + (int64_t)(head / p.group) * p.v_hs;
+    __nv_bfloat16* dst = p.out + (int64_t)q_row * p.o_ts + (int64_t)head * p.o_hs;
     float2 q[W], o[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -370,8 +402,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         for (int k = 0; next_item(k, it); ++k) {
             const int tiles = t == 0 ? it.n[0] : it.n[1];
             if (tiles == 0) continue;
-            const int row = t * kPfTile + wq * 32 + lane;
-            const int sees = p.causal ? min(it.kv_len, it.limit + row) : it.kv_len;
+            const int sees = p.causal ? min(it.kv_len, (t == 0 ? it.limit[0] : it.limit[1]) + wq * 32 + lane) : it.kv_len;
             float m = -INFINITY;                                   // M / c
             float2 l2 = make_float2(0.f, 0.f);
             bool ok = true;
@@ -446,12 +477,12 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 if (!ok) continue;
                 ++uses[t];
                 tm_fence_after();
-                const int r = wq * 32 + lane, row = t * kPfTile + r;
+                const int r = wq * 32 + lane;
                 const float l = s_l[t][r];
-                const int sees = p.causal ? min(it.kv_len, it.limit + row) : it.kv_len;
+                const int sees = p.causal ? min(it.kv_len, it.limit[t] + r) : it.kv_len;
                 const bool none = sees <= 0 || l == 0.f;           // nothing to average: zeros, whatever the product holds
                 const float2 inv2 = make_float2(1.f / l, 1.f / l);
-                __nv_bfloat16* dst = p.out + (int64_t)(it.q_row + row) * p.o_ts + (int64_t)it.head * p.o_hs;
+                __nv_bfloat16* dst = p.out + (int64_t)(it.q_row[t] + r) * p.o_ts + (int64_t)it.head[t] * p.o_hs;
                 const uint32_t o_addr = tmem + lanes + 256 + t * kPfTile;
                 float2 odd2 = make_float2(0.f, 0.f);               // 0 x (a value that is not finite) is NaN
                 uint32_t o[2][16];
@@ -473,7 +504,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         odd2 = __ffma2_rn(f, make_float2(0.f, 0.f), odd2);
                         w[e] = none ? 0u : pack2(f);
                     }
-                    if (row < it.rows) {
+                    if (r < it.rows[t]) {
                         if (p.out32) {
                             asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 16 * c), NMT_W8(w, 0) : "memory");
                         } else {
@@ -482,11 +513,10 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         }
                     }
                 }
-                const bool odd = !none && row < it.rows && odd2.x + odd2.y != 0.f;
+                const bool odd = !none && r < it.rows[t] && odd2.x + odd2.y != 0.f;
                 for (uint32_t redo = __ballot_sync(0xffffffffu, odd && l < INFINITY); redo; redo &= redo - 1) {
-                    const int src = __ffs(redo) - 1, rr = t * kPfTile + wq * 32 + src;
-                    redo_row<D>(p, it, rr, p.causal ? min(it.kv_len, it.limit + rr) : it.kv_len,
-                                p.out + (int64_t)(it.q_row + rr) * p.o_ts + (int64_t)it.head * p.o_hs);
+                    const int rr = wq * 32 + __ffs(redo) - 1;
+                    redo_row<D>(p, it.q_row[t] + rr, it.head[t], it.kv_row, p.causal ? min(it.kv_len, it.limit[t] + rr) : it.kv_len);
                 }
             }
         }
@@ -609,13 +639,13 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     continue;
                 }
                 publish(k++);
-                const int n_max = max(it.n[0], it.n[1]), kv_head = it.head / p.group;
+                const int n_max = max(it.n[0], it.n[1]);
                 auto load_q = [&](int t) {
                     if (it.n[t] == 0 || !ok) return;
                     if (q_uses[t] > 0) ok = warp_wait(&bar.q_empty[t], (q_uses[t] - 1) & 1u);
                     if (!ok) return;
                     ++q_uses[t];
-                    load(&qmap, it.head, it.q_row + t * kPfTile, q_smem + t * Shape::kTileBytes, &bar.q_full[t]);
+                    load(&qmap, it.head[t], it.q_row[t], q_smem + t * Shape::kTileBytes, &bar.q_full[t]);
                 };
                 if (ok) load_q(0);
                 for (int i = 0; i < 2 * n_max && ok; ++i, ++kv) {
@@ -629,7 +659,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     if ((i & 1) && valid < kPfTile) {
                         // Keys past the sequence's end belong to another one or to nobody, and 0 x NaN is NaN: their rows of V
                         // are cleared before anybody is told that the tile is there.
-                        load(&vmap, kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.v_raw);
+                        load(&vmap, it.kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.v_raw);
                         ok = warp_wait(&bar.v_raw, v_raws++ & 1u);
                         if (!ok) break;
                         const int from = max(valid, 0);
@@ -642,7 +672,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         if (lane == 0) mbar_arrive(&bar.kv_full[st]);
                         __syncwarp();
                     } else {
-                        load(i & 1 ? &vmap : &kmap, kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.kv_full[st]);
+                        load(i & 1 ? &vmap : &kmap, it.kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.kv_full[st]);
                     }
                     if (i == 0) load_q(1);
                 }
@@ -686,10 +716,13 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
         return NMT_ERR_SHAPE;
     if ((!cu_q && (batch != 1 || cu_k))) return NMT_ERR_SHAPE;
     if (head_dim != 64 && head_dim != 128) return NMT_ERR_UNSUPPORTED;
-    // Blocks of 256 rows: all that the batch can have (every sequence may end in a partly filled one); CTAs past the real
-    // number find nothing to do.
-    const int64_t full = (q_tokens + kPfRows - 1) / kPfRows, blocks = cu_q ? (q_tokens < full + batch - 1 ? q_tokens : full + batch - 1) : full;
-    if (q_tokens > 0x3fffffff || kv_tokens > 0x3fffffff || batch > 0x3fffffff || heads > 65535 || blocks * heads > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
+    if (q_tokens > 0x3fffffff || kv_tokens > 0x3fffffff || batch > 0x3fffffff || heads > 65535) return NMT_ERR_UNSUPPORTED;
+    // Items: two query tiles (128 rows of a head) of a sequence and kv head each.  As many as the batch can have (every
+    // sequence may end in a partly filled block and an odd tile); CTAs past the real number find nothing to do.
+    const int64_t full = (q_tokens + kPfTile - 1) / kPfTile, some = cu_q ? batch : 1;
+    const int64_t blocks = q_tokens < full + some - 1 ? q_tokens : full + some - 1, group = heads / kv_heads;
+    const int64_t items = (blocks * group + (blocks < some ? blocks : some)) / 2 * kv_heads;
+    if (blocks * heads > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
     if (q_tokens == 0 || batch == 0) return NMT_OK;
     int st;
     if ((st = check_view(q, q_tokens, q_ts, heads, q_hs)) != NMT_OK || (st = check_view(out, q_tokens, o_ts, heads, o_hs)) != NMT_OK) return st;
@@ -722,11 +755,11 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
     p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.batch = static_cast<int>(batch); p.q_tokens = static_cast<int>(q_tokens); p.kv_tokens = static_cast<int>(kv_tokens);
-    p.heads = static_cast<int>(heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
+    p.kv_heads = static_cast<int>(kv_heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
     p.out32 = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && (q_tokens == 1 || o_ts % 16 == 0) && (heads == 1 || o_hs % 16 == 0);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    const int items = static_cast<int>(blocks * heads);
-    if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, items, cs); else launch_prefill<64>(maps[0], maps[1], maps[2], p, items, cs);
+    if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, static_cast<int>(items), cs);
+    else launch_prefill<64>(maps[0], maps[1], maps[2], p, static_cast<int>(items), cs);
     return finish_launch(1);
 }
 
