@@ -95,6 +95,8 @@ class NemotronB200Error(RuntimeError):
 def load() -> C.CDLL:
     """Loads the library once and binds every prototype; raises if anything is missing."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -218,6 +218,16 @@ inline void launch_cluster_kernel(void (*kern)(KArgs...), int grid, int cluster,
     cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// Lets `kern` use up to `bytes` of dynamic shared memory, once per kernel and device: `done` is the caller's, one bit per device.
+template <typename F>
+inline void allow_smem(F* kern, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 inline int grid_for(int64_t work_items, int items_per_cta, int max_ctas) {
     int64_t g = (work_items + items_per_cta - 1) / items_per_cta;
     if (g < 1) g = 1;

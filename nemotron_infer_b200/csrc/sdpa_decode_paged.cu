@@ -20,7 +20,7 @@
 //     tensor memory, M = 128 rows for 5 heads) to a kernel that waits for HBM.
 //   * Precision.  P is split into two bf16 terms (p = hi + lo, 16 bits) against a bf16 V.  e4m3 values and the query,
 //     scaled by a power of two per head, are exact in f16 and P keeps 11 bits there.  Scores, maxima, sums, output: fp32.
-#include <cfloat>
+#include <type_traits>
 
 #include "nmt_paged.cuh"
 #include "nmt_tensormap.cuh"
@@ -508,20 +508,23 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
 
 // Joins the pieces of the units that were cut.  CTA (c - 1, r) belongs to the cut between ranges c - 1 and c; it works if
 // that is the FIRST cut inside the unit there, and joins query head r of it: pieces c - 1 (its last), c, c + 1, ...
-constexpr int kJoinThreads = 256;
+// Nothing here is long, so the chain of dependent loads counts: what cut this is -> maxima, sums and outputs, all at once.
+// A warp takes every eighth piece, a lane D / 32 columns of it; every warp works out the weights for itself.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kJoinWarps * 32)
 sdpa_decode_paged_join_kernel(const DecodeArgs p, int hpu) {
-    constexpr int SLICES = kJoinThreads / D;
-    __shared__ float s_w[kDecCtas], s_red[2][kJoinThreads / 32], s_acc[SLICES][D];
+    constexpr int CPL = D / 32, AHEAD = 5;                         // columns per lane; pieces loaded before the weights are known
+    __shared__ __align__(16) float s_acc[kJoinWarps][D];
     pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x + 1, r = blockIdx.y;
-    const int4 prev1 = p.desc[1], mine0 = p.desc[2 * c];
-    const int ctas = prev1.x;
-    const int64_t total = ((int64_t)prev1.w << 32) | (uint32_t)prev1.z;
+    const int4 line = p.desc[1], cut = p.desc[2 * c];
+    const int ctas = line.x;
+    const int64_t total = ((int64_t)line.w << 32) | (uint32_t)line.z;
     if (c < ctas) {
         const int64_t start = (int64_t)c * total / ctas, start_prev = (int64_t)(c - 1) * total / ctas;
-        const int f = mine0.z, tiles = mine0.w, b = mine0.x, unit = mine0.y;
+        const int f = cut.z, tiles = cut.w, b = cut.x, unit = cut.y;
         const int head = unit / p.chunks, q0 = (unit % p.chunks) * hpu, heads = min(hpu, p.group - q0);
         if (f > 0 && f <= start - start_prev && r < heads) {
             const int64_t unit_end = start + (tiles - f);
@@ -529,34 +532,44 @@ sdpa_decode_paged_join_kernel(const DecodeArgs p, int hpu) {
             const int n = last - (c - 1) + 1;
             const int slot0 = f == start - start_prev ? 0 : 1;
             auto piece = [&](int i) { return ((size_t)(c - 1 + i) * 2 + (i == 0 ? slot0 : 0)) * hpu + r; };
-            float top = -INFINITY;
-            for (int i = threadIdx.x; i < n; i += kJoinThreads) top = fmaxf(top, p.ml[piece(i)].x);
-            top = warp_max(top);
-            if ((threadIdx.x & 31) == 0) s_red[0][threadIdx.x >> 5] = top;
-            __syncthreads();
-            for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[0][w]);
-            float sum = 0.f;
-            for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-                const float2 ml = p.ml[piece(i)];
-                const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-                s_w[i] = w;
-                sum += w * ml.y;
-            }
-            sum = warp_sum(sum);
-            if ((threadIdx.x & 31) == 0) s_red[1][threadIdx.x >> 5] = sum;
-            __syncthreads();
-            sum = 0.f;
-            for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[1][w];
-            const int d = threadIdx.x % D, slice = threadIdx.x / D;
-            float acc = 0.f;
-#pragma unroll 8
-            for (int i = slice; i < n; i += SLICES) acc = fmaf(s_w[i], p.o[piece(i) * D + d], acc);
-            s_acc[slice][d] = acc;
-            __syncthreads();
-            if (slice == 0) {
+            using Cols = typename std::conditional<D == 128, float4, float2>::type;
+            Cols ahead[AHEAD];
 #pragma unroll
-                for (int s = 1; s < SLICES; ++s) acc += s_acc[s][d];
-                p.out[b * p.o_ss + (int64_t)(head * p.group + q0 + r) * p.o_hs + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+            for (int k = 0; k < AHEAD; ++k) {
+                const int i = warp + k * kJoinWarps;
+                if (i < n) ahead[k] = *reinterpret_cast<const Cols*>(p.o + piece(i) * D + lane * CPL);
+            }
+            float top = -INFINITY, sum = 0.f;
+            for (int i = lane; i < n; i += 32) {
+                const float2 ml = p.ml[piece(i)];
+                const float t = fmaxf(top, ml.x);
+                if (t > -INFINITY) sum = sum * ex2(top - t) + (ml.x == -INFINITY ? 0.f : ml.y * ex2(ml.x - t));
+                top = t;
+            }
+            const float all = warp_max(top);
+            sum = warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - all));
+            float acc[CPL];
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) acc[e] = 0.f;
+            auto add = [&](int i, const Cols& v) {
+                const float m = p.ml[piece(i)].x, w = m == -INFINITY ? 0.f : ex2(m - all);
+                const float* x = reinterpret_cast<const float*>(&v);
+#pragma unroll
+                for (int e = 0; e < CPL; ++e) acc[e] = fmaf(w, x[e], acc[e]);
+            };
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (warp + k * kJoinWarps < n) add(warp + k * kJoinWarps, ahead[k]);
+#pragma unroll 4
+            for (int i = warp + AHEAD * kJoinWarps; i < n; i += kJoinWarps) add(i, *reinterpret_cast<const Cols*>(p.o + piece(i) * D + lane * CPL));
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) s_acc[warp][lane * CPL + e] = acc[e];
+            __syncthreads();
+            if (threadIdx.x < D) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < kJoinWarps; ++w) v += s_acc[w][threadIdx.x];
+                p.out[b * p.o_ss + (int64_t)(head * p.group + q0 + r) * p.o_hs + threadIdx.x] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
             }
         }
     }
@@ -568,12 +581,13 @@ static int decode_nt(int64_t group) { return group > 8 ? 2 : 1; }
 template <int D, bool E4M3, int NT>
 static void launch_decode(const CUtensorMap& km, const CUtensorMap& vm, const DecodeArgs& p, int ctas, cudaStream_t st) {
     auto kern = sdpa_decode_paged_kernel<D, E4M3, NT>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kDecSmem));
+    static std::atomic<uint64_t> allowed{0};
+    allow_smem(kern, kDecSmem, allowed);
     launch_kernel(kern, ctas, kDecThreads, kDecSmem, st, km, vm, p);
     if (ctas > 1) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(ctas - 1), static_cast<unsigned>(p.group < NT * 8 ? p.group : NT * 8));
-        cfg.blockDim = dim3(kJoinThreads);
+        cfg.blockDim = dim3(kJoinWarps * 32);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -699,7 +699,8 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
 template <int D>
 static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, int items, cudaStream_t st) {
     auto kern = sdpa_prefill_kernel<D>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PfShape<D>::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    allow_smem(kern, PfShape<D>::kSmem, allowed);
     launch_kernel(kern, items, kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
 }
 

@@ -253,6 +253,12 @@ def sdpa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
     return out
 
 
+# Single-token steps are short enough for the host side to count: the current device and stream come from the bindings below
+# torch.cuda's wrappers where this torch has them (5 us less per call).
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _on_device(fn):
     """The operators over strided views and caches may be called with tensors of a device that is not the current one: they
     run on that device, on its current stream."""
@@ -261,7 +267,7 @@ def _on_device(fn):
         dev = first.device
         if dev.type != "cuda":
             raise ValueError("nemotron_infer_b200 operators run on CUDA tensors only (no CPU fallback)")
-        if dev.index == torch.cuda.current_device():
+        if dev.index == _current_device():
             return fn(first, *args, **kwargs)
         with torch.cuda.device(dev):
             return fn(first, *args, **kwargs)
@@ -286,6 +292,8 @@ def _view3(t: torch.Tensor, name: str, rows: int | None, heads: int | None, dim:
 def _result3(t: torch.Tensor, name: str, rows: int, heads: int, dim: int, dev) -> tuple[int, int]:
     """The same for a tensor that is written: no two of its rows may share memory."""
     rs, hs = _view3(t, name, rows, heads, dim, dev)
+    if t.is_contiguous():
+        return rs, hs
     spans = sorted(((abs(s), n) for s, n in ((rs, rows), (hs, heads)) if n > 1))
     need = dim
     for s, n in spans:
@@ -380,14 +388,14 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             raise ValueError("q is only rotated: it needs rope")
         qs = _view3(q, "q", T, None, c.head_dim, dev)
         q_heads = q.shape[1]
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+        q_out = q.new_empty(q.shape) if q_out is None else q_out
         os = _result3(q_out, "q_out", T, q_heads, c.head_dim, dev)
     elif q_out is not None:
         raise ValueError("q_out without q")
     _lib.check(_lib.load().nmt_kv_append_paged_bf16(
         c, cu, T, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], None if rope is None else rope.data_ptr(), rows, rot,
         1 if interleaved else 0, None if q is None else q.data_ptr(), qs[0], qs[1], q_heads, None if q is None else q_out.data_ptr(),
-        os[0], os[1], None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), _stream()), "kv_append_paged")
+        os[0], os[1], None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), _raw_stream(dev.index)), "kv_append_paged")
     return q_out
 
 
@@ -414,7 +422,7 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         raise ValueError("q must be bf16 [batch, heads, head_dim]")
     heads = q.shape[1]
     qs = _view3(q, "q", c.batch, heads, c.head_dim, dev)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    out = q.new_empty(q.shape) if out is None else out
     os = _result3(out, "out", c.batch, heads, c.head_dim, dev)
     lib = _lib.load()
     if workspace is None:
@@ -425,7 +433,7 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     _lib.check(lib.nmt_sdpa_decode_paged_bf16(c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads,
                                               c.head_dim ** -0.5 if scale is None else scale,
                                               None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), workspace.data_ptr(),
-                                              _stream()), "sdpa_decode_paged")
+                                              _raw_stream(dev.index)), "sdpa_decode_paged")
     return out
 
 
@@ -458,11 +466,11 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: 
             raise ValueError("with cu_seqlens alone, k and v have q's rows")
     elif cu_seqlens_k is not None:
         raise ValueError("cu_seqlens_k without cu_seqlens")
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    out = q.new_empty(q.shape) if out is None else out
     os = _result3(out, "out", T, heads, dim, dev)
     _lib.check(_lib.load().nmt_sdpa_prefill_bf16(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
                                                  out.data_ptr(), os[0], os[1], cu, cu_k, batch, T, T_k, heads, kv_heads, dim,
-                                                 dim ** -0.5 if scale is None else scale, 1 if causal else 0, _stream()), "sdpa_prefill")
+                                                 dim ** -0.5 if scale is None else scale, 1 if causal else 0, _raw_stream(dev.index)), "sdpa_prefill")
     return out
 
 
