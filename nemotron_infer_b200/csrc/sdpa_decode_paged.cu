@@ -7,8 +7,10 @@
 //   * Balance.  A unit is (sequence, kv head, up to 16 of its query heads); it is cut into tiles of 16 KB of K and 16 KB of
 //     V (64 to 256 positions).  All tiles of the batch form one line, sequence by sequence, and each of up to 296 CTAs (two
 //     per SM) takes an equal piece of it, whatever the lengths are: every CTA sums the lengths itself (they are only known
-//     on the device), so a captured graph follows them.  A unit that one CTA holds whole is finished there; a cut one
-//     leaves (maximum, sum, output) per piece in the workspace and a second launch joins the pieces.
+//     on the device), so a captured graph follows them.  A unit counts for one tile more than it has, for what its start
+//     and its end take (query, joining the warps): without that, CTAs that held 15 sequences of a few tokens each ran for
+//     46 us beside others' 30.  A unit that one CTA holds whole is finished there; a cut one leaves (maximum, sum, output)
+//     per piece in the workspace and a second launch joins the pieces.
 //   * Copies.  A producer warp looks up the pages and brings them in with tensor-map copies (one box per page and 128
 //     bytes of row, swizzled so that ldmatrix reads without bank conflicts) through a ring of three tiles per CTA: 192 KB
 //     per SM on their way.  A page id out of range goes out as a coordinate out of range, which the copy fills with zeros.
@@ -35,6 +37,7 @@ constexpr int kDecThreads = (kDecWarps + 1) * 32;
 constexpr int kDecStages = 3;
 constexpr int kTileBytes = 16384;                                  // of K, and as much of V
 constexpr int kDecCtas = 2 * kSmCount;
+constexpr int kUnitCost = 1;                                       // what a unit counts for beside its tiles
 constexpr int kMergeCols = 68;                                     // 64 columns + 4: head rows of the merge buffer hit different banks
 constexpr size_t kDecMergeBytes = kDecWarps * 8 * kMergeCols * sizeof(float);
 constexpr size_t kDecSmem = 1024 + (size_t)kDecStages * 2 * kTileBytes + kDecMergeBytes;
@@ -121,7 +124,7 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
     extern __shared__ __align__(1024) uint8_t smem_d[];
     __shared__ uint64_t s_full[kDecStages], s_empty[kDecStages];
     __shared__ int64_t s_sum[kDecThreads / 32];
-    __shared__ int64_t s_start[2];                                 // first tile of this CTA, inside sequence s_b
+    __shared__ int64_t s_start;                                    // where this CTA starts inside sequence s_b
     __shared__ int s_b;
     __shared__ float s_m[kDecWarps][HPU], s_l[kDecWarps][HPU];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -142,7 +145,7 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
     for (int b = b_lo; b < b_hi; ++b) {
         const int cap = p.max_pages << p.page_shift, raw = p.seq_lens[b];
         too_long |= raw > cap;
-        mine += max(1, (min(max(raw, 0), cap) + TK - 1) >> p.tile_shift);
+        mine += kUnitCost + max(1, (min(max(raw, 0), cap) + TK - 1) >> p.tile_shift);
     }
     if (too_long && blockIdx.x == 0 && p.err_flag) *p.err_flag = 1;
     mine *= units_per_seq;
@@ -160,15 +163,15 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
         if (w < warp) before += s_sum[w];
         total += s_sum[w];
     }
-    const int ctas = static_cast<int>(min((int64_t)gridDim.x, total));     // every one of them has at least one tile
+    const int ctas = static_cast<int>(min((int64_t)gridDim.x, total));
     const int64_t begin = (int64_t)blockIdx.x * total / ctas, end = (int64_t)(blockIdx.x + 1) * total / ctas;
     const bool active = (int)blockIdx.x < ctas;
     if (active && begin >= before && begin < before + mine) {
         int64_t at = before;
         for (int b = b_lo; b < b_hi; ++b) {
             const int len = min(max(p.seq_lens[b], 0), p.max_pages << p.page_shift);
-            const int64_t n = (int64_t)max(1, (len + TK - 1) >> p.tile_shift) * units_per_seq;
-            if (begin < at + n) { s_b = b; s_start[0] = begin - at; break; }
+            const int64_t n = (int64_t)(kUnitCost + max(1, (len + TK - 1) >> p.tile_shift)) * units_per_seq;
+            if (begin < at + n) { s_b = b; s_start = begin - at; break; }
             at += n;
         }
     }
@@ -177,9 +180,18 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
         Cursor c;
         c.b = s_b;
         c.seat(p);
-        c.unit = static_cast<int>(s_start[0] / c.tiles);
-        c.tile = static_cast<int>(s_start[0] % c.tiles);
-        int64_t left = end - begin;
+        // A place on the line is kUnitCost places of a unit's own, where nothing is cut, then its tiles.
+        c.unit = static_cast<int>(s_start / (kUnitCost + c.tiles));
+        int64_t left = end - begin;                                // places of the line still to go
+        {
+            const int at = static_cast<int>(s_start % (kUnitCost + c.tiles));
+            c.tile = max(at - kUnitCost, 0);
+            if (at <= kUnitCost) left += at;                       // a cut among a unit's own places is one before all of them
+        }
+        // tiles of the unit the cursor is in that are this CTA's: none when the range ends among its own places
+        auto share = [&](int64_t places, const Cursor& k) {
+            return static_cast<int>(min((int64_t)(k.tiles - k.tile), k.tile == 0 ? places - kUnitCost : places));
+        };
         if (threadIdx.x == 0) {
             p.desc[2 * blockIdx.x] = make_int4(c.b, c.unit, c.tile, c.tiles);
             p.desc[2 * blockIdx.x + 1] = make_int4(ctas, 0, static_cast<int>(total & 0xffffffff), static_cast<int>(total >> 32));
@@ -189,32 +201,36 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
             const int page_rows = 1 << p.page_shift, box_rows = min(page_rows, TK);
             int n = 0;
             bool ok = true;
-            for (; left > 0 && ok; --left, ++n) {
-                const int stage = n % kDecStages;
-                const int pos = c.tile * TK, valid = min(TK, c.len - pos), head = c.unit / p.chunks;
-                const int pages = valid > 0 ? (valid + box_rows - 1) / box_rows : 0;           // at most TK / 8 <= 32
-                int page = p.num_pages;
-                if (lane < pages) {
-                    page = p.page_table[(int64_t)c.b * p.max_pages + (pos >> p.page_shift) + lane];
-                    if (page < 0 || page >= p.num_pages) {
-                        page = p.num_pages;                        // out of the map's range: the copy fills in zeros
-                        if (p.err_flag) *p.err_flag = 1;
+            for (int take; ok && (take = share(left, c)) > 0;) {
+                left -= take + (c.tile == 0 ? kUnitCost : 0);
+                for (; take > 0; --take, ++n) {
+                    const int stage = n % kDecStages;
+                    const int pos = c.tile * TK, valid = min(TK, c.len - pos), head = c.unit / p.chunks;
+                    const int pages = valid > 0 ? (valid + box_rows - 1) / box_rows : 0;           // at most TK / 8 <= 32
+                    int page = p.num_pages;
+                    if (lane < pages) {
+                        page = p.page_table[(int64_t)c.b * p.max_pages + (pos >> p.page_shift) + lane];
+                        if (page < 0 || page >= p.num_pages) {
+                            page = p.num_pages;                        // out of the map's range: the copy fills in zeros
+                            if (p.err_flag) *p.err_flag = 1;
+                        }
                     }
-                }
-                if (n >= kDecStages) ok = mbar_wait(&s_empty[stage], static_cast<uint32_t>(n / kDecStages - 1) & 1u);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(&s_full[stage], pages * box_rows * ROWB * 2);
-                __syncwarp();
-                if (lane < pages) {
-                    const uint32_t kd = ring + stage * 2 * kTileBytes + lane * box_rows * CH, vd = kd + kTileBytes;
-                    const int row = pos & (page_rows - 1);
+                    if (n >= kDecStages) ok = mbar_wait(&s_empty[stage], static_cast<uint32_t>(n / kDecStages - 1) & 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&s_full[stage], pages * box_rows * ROWB * 2);
+                    __syncwarp();
+                    if (lane < pages) {
+                        const uint32_t kd = ring + stage * 2 * kTileBytes + lane * box_rows * CH, vd = kd + kTileBytes;
+                        const int row = pos & (page_rows - 1);
 #pragma unroll
-                    for (int ch = 0; ch < NCH; ++ch) tma_page_box(kd + ch * TK * CH, &kmap, ch * (D / NCH), row, head, page, &s_full[stage]);
+                        for (int ch = 0; ch < NCH; ++ch) tma_page_box(kd + ch * TK * CH, &kmap, ch * (D / NCH), row, head, page, &s_full[stage]);
 #pragma unroll
-                    for (int ch = 0; ch < NCH; ++ch) tma_page_box(vd + ch * TK * CH, &vmap, ch * (D / NCH), row, head, page, &s_full[stage]);
+                        for (int ch = 0; ch < NCH; ++ch) tma_page_box(vd + ch * TK * CH, &vmap, ch * (D / NCH), row, head, page, &s_full[stage]);
+                    }
+                    ++c.tile;
                 }
-                if (++c.tile == c.tiles) c.next_unit(p);
+                if (c.tile == c.tiles) c.next_unit(p);
             }
             for (int s = max(0, n - kDecStages); s < n; ++s) mbar_wait(&s_full[s % kDecStages], static_cast<uint32_t>(s / kDecStages) & 1u);
         } else {
@@ -223,7 +239,7 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
             bool ok = true;                                        // a wait that ran out: results void, control flow unchanged
             int n = 0;
             bool first_fragment = true;
-            while (left > 0) {
+            for (int take; (take = share(left, c)) > 0;) {
                 const int head = c.unit / p.chunks, q0 = (c.unit % p.chunks) * HPU, heads = min(HPU, p.group - q0);
                 // the query heads as B operand: column g of tile nt is head q0 + nt * 8 + g
                 uint32_t qf[NT][KS][2];
@@ -276,7 +292,6 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
                     m[nt][0] = m[nt][1] = -INFINITY;
                     l[nt][0] = l[nt][1] = 0.f;
                 }
-                const int take = static_cast<int>(min((int64_t)(c.tiles - c.tile), left));
                 for (int i = 0; i < take; ++i, ++n) {
                     const int stage = n % kDecStages;
                     const int valid = c.len - (c.tile + i) * TK;
@@ -496,7 +511,7 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
                         }
                         consumer_barrier();
                     }
-                left -= take;
+                left -= take + (c.tile == 0 ? kUnitCost : 0);
                 c.tile += take;
                 first_fragment = false;
                 if (c.tile == c.tiles) c.next_unit(p);
@@ -530,7 +545,7 @@ sdpa_decode_paged_join_kernel(const DecodeArgs p, int hpu) {
             const int64_t unit_end = start + (tiles - f);
             const int last = static_cast<int>((unit_end * ctas + total - 1) / total) - 1;       // range that holds its last tile
             const int n = last - (c - 1) + 1;
-            const int slot0 = f == start - start_prev ? 0 : 1;
+            const int slot0 = f + kUnitCost >= start - start_prev ? 0 : 1;         // was the unit the first of range c - 1
             auto piece = [&](int i) { return ((size_t)(c - 1 + i) * 2 + (i == 0 ? slot0 : 0)) * hpu + r; };
             using Cols = typename std::conditional<D == 128, float4, float2>::type;
             Cols ahead[AHEAD];
@@ -656,7 +671,7 @@ int nmt_sdpa_decode_paged_bf16(const nmt_paged_cache* c, const void* q, int64_t 
     p.scale_step = c->scale_count > 1 ? 1 : 0;
     p.tile_shift = log2_of(tile);
     // no more CTAs than there can be tiles
-    const int64_t cap = (c->max_pages * c->page_size + tile - 1) / tile, per_seq = cap * c->kv_heads * p.chunks;
+    const int64_t cap = (c->max_pages * c->page_size + tile - 1) / tile, per_seq = (cap + kUnitCost) * c->kv_heads * p.chunks;
     const int ctas = per_seq >= kDecCtas || per_seq * c->batch >= kDecCtas ? kDecCtas : static_cast<int>(per_seq * c->batch);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
 #define NMT_DEC_NT(D, E) do { if (nt == 2) launch_decode<D, E, 2>(km, vm, p, ctas, cs); else launch_decode<D, E, 1>(km, vm, p, ctas, cs); } while (0)
