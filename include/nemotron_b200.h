@@ -265,7 +265,7 @@ typedef struct nmt_paged_cache {
 
 /* Writes the keys and values of `tokens` new tokens into their pages, and rotates K (and Q) by position on the way.
  *   cu_new     device int32 [batch + 1], ascending: the tokens of sequence b are rows cu_new[b] .. cu_new[b + 1] - 1 of k,
- *              v and q, and its LAST one has position seq_lens[b] - 1.  Rows behind cu_new[batch] are padding: not read,
+ *              v and q, and its LAST one has position seq_lens[b] - 1.  Rows behind cu_new[batch] are padding: not used,
  *              nothing written for them.  NULL: one token per sequence (tokens == batch), the decode step.
  *   k, v       bf16 [tokens][kv_heads][head_dim] with any token and head strides (in elements, multiples of 8)
  *   rope       NULL: no rotation.  Else fp32 [rope_rows][rot_dim]: row p holds rot_dim / 2 cosines, then as many sines, of

@@ -4,17 +4,18 @@
 //   K'[t, h] = R(pos) K[t, h],  Q'[t, h] = R(pos) Q[t, h]      R(pos): pairs (x_i, x_j) -> (x_i c - x_j s, x_j c + x_i s)
 //   k_cache[page_table[b, pos / P], h, pos % P] = round(K'[t, h] / k_scale),  the same for V without the rotation
 //
-// Pure streaming: every row is read once and written once (5 KB per token without Q at 8 heads of 128 in bf16, 24.5 KB
-// with 40 rotated query heads).  An item is the 16 elements of a head that turn together - two 16-byte vectors, half a
-// rotation apart or side by side - so no lane needs another lane's data and every access is 16 bytes wide.  A warp owns
-// up to 128 items of ONE token, four per lane with all eight loads issued before the first use; the sequence search, the
-// page lookup and the cosine / sine row are then per warp, not per head.
+// Pure streaming: every row is read once and written once (8 KB per token without Q at 8 heads of 128 in bf16, 28 KB with 40
+// rotated query heads).  An item is two 16-byte vectors of a head: the two that turn together where pairs are half a rotation
+// apart, otherwise the same place in the two halves of what is left - so no lane needs another lane's data, every access
+// is 16 bytes wide and neighbouring lanes touch neighbouring vectors.  A warp owns up to 64 items of ONE token, two per
+// lane with all four loads issued before the first use; the sequence search, the page lookup and the cosine / sine row
+// are then per warp, not per head.  32 items of one kind (K, V or Q) at a time: what a lane does is the same all over the warp.
 #include "nmt_paged.cuh"
 
 namespace nmt {
 
 constexpr int kAppendWarps = 4;
-constexpr int kItemsPerLane = 4;
+constexpr int kItemsPerLane = 2;                                  // 4 took 3.5 us instead of 2.9 for a step of 32 tokens, the same for prompts
 
 struct AppendArgs {
     const int32_t* cu;
@@ -30,14 +31,16 @@ struct AppendArgs {
     int batch, tokens, kv_heads, q_heads, num_pages, max_pages, page_shift, rope_rows, rot, scale_step, warps_per_token;
 };
 
-// (a, b) -> (a c - b s, b c + a s) for the pairs of one item.  INTERLEAVED: a pair is two neighbours of one vector.
+// (a, b) -> (a c - b s, b c + a s) for the pairs of one item, whose vectors start at elements off_a and off_b of the head.
+// INTERLEAVED: a pair is two neighbours of one vector.
 template <bool INTERLEAVED>
-__device__ __forceinline__ void rotate_item(float (&a)[8], float (&b)[8], const float* __restrict__ row, int half, int first_pair) {
+__device__ __forceinline__ void rotate_item(float (&a)[8], float (&b)[8], const float* __restrict__ row, int half, int off_a, int off_b) {
+    const int p0 = INTERLEAVED ? off_a / 2 : off_a, p1 = INTERLEAVED ? off_b / 2 : off_a + 4;    // pairs 0-3 and 4-7
     float c[8], s[8];
-    *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(row + first_pair));
-    *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(row + first_pair + 4));
-    *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(row + half + first_pair));
-    *reinterpret_cast<float4*>(s + 4) = __ldg(reinterpret_cast<const float4*>(row + half + first_pair + 4));
+    *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(row + p0));
+    *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(row + p1));
+    *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(row + half + p0));
+    *reinterpret_cast<float4*>(s + 4) = __ldg(reinterpret_cast<const float4*>(row + half + p1));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float& x = INTERLEAVED ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
@@ -48,15 +51,77 @@ __device__ __forceinline__ void rotate_item(float (&a)[8], float (&b)[8], const 
     }
 }
 
+// x / s for the e4m3 rounding that follows, as x * hi + x * lo with 1 / s = hi + lo to 2^-39: hi has 16 bits, so that a
+// bf16 x times hi is exact and the sum is rounded once.  A quotient that fp32 holds - a tie between two e4m3 values, above
+// all - comes out exactly, for two instructions per pair of elements (a division takes about ten each).  lo is positive
+// and never zero (hi is cut from a value just below 1 / s): an infinity stays one.
+__device__ __noinline__ uint2 quantize_by_division(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float s) {
+    return make_uint2(e4m3x2_rn(__fdiv_rn(x0, s), __fdiv_rn(x1, s)) | (e4m3x2_rn(__fdiv_rn(x2, s), __fdiv_rn(x3, s)) << 16),
+                      e4m3x2_rn(__fdiv_rn(x4, s), __fdiv_rn(x5, s)) | (e4m3x2_rn(__fdiv_rn(x6, s), __fdiv_rn(x7, s)) << 16));
+}
+struct Divisor {
+    float s, hi, lo;
+    bool fits;                                                     // otherwise a product could leave fp32's range: divide
+    __device__ __forceinline__ explicit Divisor(float scale) : s(scale) {
+        const float r = __frcp_rn(s);
+        hi = __uint_as_float(__float_as_uint(r * (1.f - 0x1p-20f)) & 0xffffff00u);
+        lo = __fmaf_rn(-hi, s, 1.f) * r;
+        fits = s >= 0x1p-15f && s <= 0x1p100f;
+    }
+    // Eight elements -> eight bytes.
+    __device__ __forceinline__ uint2 quantize(const float (&x)[8]) const {
+        if (!fits) return quantize_by_division(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s);
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 v = make_float2(x[2 * e], x[2 * e + 1]);
+            const float2 w = __ffma2_rn(v, make_float2(lo, lo), __fmul2_rn(v, make_float2(hi, hi)));
+            q[2 * e] = w.x;
+            q[2 * e + 1] = w.y;
+        }
+        return make_uint2(e4m3x2_rn(q[0], q[1]) | (e4m3x2_rn(q[2], q[3]) << 16), e4m3x2_rn(q[4], q[5]) | (e4m3x2_rn(q[6], q[7]) << 16));
+    }
+};
+
 template <int D, bool E4M3, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppendWarps * 32)
+__global__ void __launch_bounds__(kAppendWarps * 32, 10)    // 48 registers: loads in flight count, 16,384 tokens into e4m3 25.8 -> 24.0 us
 kv_append_kernel(const AppendArgs p) {
     constexpr int IPH = D / 16;                                    // items per head
     pdl_wait();
     const int lane = threadIdx.x & 31;
-    const int64_t gw = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
-    const int t = static_cast<int>(gw / p.warps_per_token), part = static_cast<int>(gw % p.warps_per_token);
+    const uint32_t gw = blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+    const int t = static_cast<int>(gw / p.warps_per_token), part = static_cast<int>(gw - t * p.warps_per_token);
     if (t >= p.tokens) return;
+    const int n_kv = p.kv_heads * IPH, n_q = p.q_heads * IPH, half = p.rot >> 1;
+    const int kv_slots = (n_kv + 31) >> 5;                         // groups of 32 items of K, as many of V, the rest Q
+    uint4 va[kItemsPerLane], vb[kItemsPerLane];
+    // item `in` of a kind: head, and where in the head its two vectors start
+    auto place = [&](int kind, int in, int& h, int& off_a, int& off_b, bool& turn) {
+        h = in / IPH;
+        const int j = in % IPH;
+        turn = kind != 1 && j * 16 < p.rot;
+        const int base = turn || kind == 1 ? 0 : p.rot, span = turn ? p.rot : D - base;       // the part of the head that it belongs to
+        off_a = base + (j * 8 - base / 2);
+        off_b = off_a + span / 2;
+    };
+    auto kind_of = [&](int slot, int& in, bool& have) {
+        const int kind = slot < kv_slots ? 0 : slot < 2 * kv_slots ? 1 : 2;
+        in = (slot - kind * kv_slots) * 32 + lane;
+        have = in < (kind == 2 ? n_q : n_kv);
+        return kind;
+    };
+    // the data first: it is on its way while the warp finds out where it goes (rows of padding are read, and then left)
+#pragma unroll
+    for (int i = 0; i < kItemsPerLane; ++i) {
+        int in, h, off_a, off_b;
+        bool have, turn;
+        const int kind = kind_of(part * kItemsPerLane + i, in, have);
+        if (!have) continue;
+        place(kind, in, h, off_a, off_b, turn);
+        const __nv_bfloat16* src = kind == 0 ? p.k + t * p.k_ts + h * p.k_hs : kind == 1 ? p.v + t * p.v_ts + h * p.v_hs : p.q + t * p.q_ts + h * p.q_hs;
+        va[i] = ld_stream(reinterpret_cast<const uint4*>(src + off_a));
+        vb[i] = ld_stream(reinterpret_cast<const uint4*>(src + off_b));
+    }
     int b = t, last = t + 1;
     if (p.cu) {
         b = find_segment(p.cu, p.batch, t);
@@ -74,65 +139,37 @@ kv_append_kernel(const AppendArgs p) {
         return;
     }
     const int slot = static_cast<int>(pos) & ((1 << p.page_shift) - 1);
-    const int n_kv = p.kv_heads * IPH, n_all = 2 * n_kv + p.q_heads * IPH, half = p.rot >> 1;
     const float* row = p.rope ? p.rope + pos * p.rot : nullptr;
-    uint4 va[kItemsPerLane], vb[kItemsPerLane];
-    int off_a[kItemsPerLane], off_b[kItemsPerLane];
 #pragma unroll
     for (int i = 0; i < kItemsPerLane; ++i) {
-        const int item = (part * kItemsPerLane + i) * 32 + lane;
-        if (item >= n_all) continue;
-        const int kind = item < n_kv ? 0 : item < 2 * n_kv ? 1 : 2;  // K, V, Q
-        const int in = item - kind * n_kv, h = in / IPH, j = in % IPH;
-        // the two vectors of item j: half a rotation apart while they are rotated (and pairs are not neighbours), else side by side
-        const bool split = !INTERLEAVED && kind != 1 && j * 16 < p.rot;
-        off_a[i] = split ? j * 8 : j * 16;
-        off_b[i] = split ? half + j * 8 : j * 16 + 8;
-        const __nv_bfloat16* src = kind == 0 ? p.k + t * p.k_ts + h * p.k_hs : kind == 1 ? p.v + t * p.v_ts + h * p.v_hs : p.q + t * p.q_ts + h * p.q_hs;
-        va[i] = ld_stream(reinterpret_cast<const uint4*>(src + off_a[i]));
-        vb[i] = ld_stream(reinterpret_cast<const uint4*>(src + off_b[i]));
-    }
-#pragma unroll
-    for (int i = 0; i < kItemsPerLane; ++i) {
-        const int item = (part * kItemsPerLane + i) * 32 + lane;
-        if (item >= n_all) continue;
-        const int kind = item < n_kv ? 0 : item < 2 * n_kv ? 1 : 2;
-        const int in = item - kind * n_kv, h = in / IPH, j = in % IPH;
-        const bool turn = kind != 1 && j * 16 < p.rot;
+        int in, h, off_a, off_b;
+        bool have, turn;
+        const int kind = kind_of(part * kItemsPerLane + i, in, have);
+        if (!have) continue;
+        place(kind, in, h, off_a, off_b, turn);
         float a[8], c[8];
         if (turn || E4M3) {
             unpack8(va[i], a);
             unpack8(vb[i], c);
         }
-        if (turn) {
-            rotate_item<INTERLEAVED>(a, c, row, half, j * 8);
-            if (!E4M3 || kind == 2) { va[i] = pack8(a); vb[i] = pack8(c); }
-        }
+        if (turn) rotate_item<INTERLEAVED>(a, c, row, half, off_a, off_b);
+        if (turn && (!E4M3 || kind == 2)) { va[i] = pack8(a); vb[i] = pack8(c); }
         if (kind == 2) {
             __nv_bfloat16* dst = p.q_out + t * p.qo_ts + h * p.qo_hs;
-            st_stream(reinterpret_cast<uint4*>(dst + off_a[i]), va[i]);
-            st_stream(reinterpret_cast<uint4*>(dst + off_b[i]), vb[i]);
+            st_stream(reinterpret_cast<uint4*>(dst + off_a), va[i]);
+            st_stream(reinterpret_cast<uint4*>(dst + off_b), vb[i]);
             continue;
         }
-        uint8_t* base = kind == 0 ? p.k_cache : p.v_cache;
         const int64_t at = (int64_t)page * (kind == 0 ? p.k_page : p.v_page) + ((int64_t)(h << p.page_shift) + slot) * D;
+        uint8_t* dst = (kind == 0 ? p.k_cache : p.v_cache) + at * (E4M3 ? 1 : 2);
         if (!E4M3) {
-            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(base) + at;
-            *reinterpret_cast<uint4*>(dst + off_a[i]) = va[i];
-            *reinterpret_cast<uint4*>(dst + off_b[i]) = vb[i];
+            *reinterpret_cast<uint4*>(dst + 2 * off_a) = va[i];
+            *reinterpret_cast<uint4*>(dst + 2 * off_b) = vb[i];
         } else {
             const float* sc = kind == 0 ? p.k_scale : p.v_scale;
-            const float s = sc ? __ldg(sc + h * p.scale_step) : 1.f;
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                w[e] = e4m3x2_rn(__fdiv_rn(a[4 * e], s), __fdiv_rn(a[4 * e + 1], s)) |
-                       (e4m3x2_rn(__fdiv_rn(a[4 * e + 2], s), __fdiv_rn(a[4 * e + 3], s)) << 16);
-                w[2 + e] = e4m3x2_rn(__fdiv_rn(c[4 * e], s), __fdiv_rn(c[4 * e + 1], s)) |
-                           (e4m3x2_rn(__fdiv_rn(c[4 * e + 2], s), __fdiv_rn(c[4 * e + 3], s)) << 16);
-            }
-            *reinterpret_cast<uint2*>(base + at + off_a[i]) = make_uint2(w[0], w[1]);
-            *reinterpret_cast<uint2*>(base + at + off_b[i]) = make_uint2(w[2], w[3]);
+            const Divisor by(sc ? __ldg(sc + h * p.scale_step) : 1.f);
+            *reinterpret_cast<uint2*>(dst + off_a) = by.quantize(a);
+            *reinterpret_cast<uint2*>(dst + off_b) = by.quantize(c);
         }
     }
     pdl_trigger();
@@ -172,10 +209,10 @@ int nmt_kv_append_paged_bf16(const nmt_paged_cache* c, const int32_t* cu_new, in
     p.q_heads = static_cast<int>(q_heads); p.num_pages = static_cast<int>(c->num_pages); p.max_pages = static_cast<int>(c->max_pages);
     p.page_shift = log2_of(c->page_size); p.rope_rows = static_cast<int>(rope_rows); p.rot = rope ? static_cast<int>(rot_dim) : 0;
     p.scale_step = c->scale_count > 1 ? 1 : 0;
-    const int64_t items = (2 * c->kv_heads + q_heads) * (c->head_dim / 16);
-    p.warps_per_token = static_cast<int>((items + 32 * kItemsPerLane - 1) / (32 * kItemsPerLane));
+    const int64_t iph = c->head_dim / 16, slots = 2 * ((c->kv_heads * iph + 31) / 32) + (q_heads * iph + 31) / 32;
+    p.warps_per_token = static_cast<int>((slots + kItemsPerLane - 1) / kItemsPerLane);
     const int64_t ctas = (tokens * p.warps_per_token + kAppendWarps - 1) / kAppendWarps;
-    if (ctas > 0x7fffffff) return NMT_ERR_UNSUPPORTED;
+    if (ctas > 0x3fffffff / kAppendWarps) return NMT_ERR_UNSUPPORTED;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     const bool e4m3 = c->dtype == NMT_CACHE_E4M3;
 #define NMT_APPEND(D, E, I) launch_kernel(kv_append_kernel<D, E, I>, static_cast<int>(ctas), kAppendWarps * 32, 0, cs, p)

@@ -101,6 +101,11 @@ __device__ __forceinline__ bool mbar_wait_now(uint64_t* bar, uint32_t parity) {
     return false;
 }
 
+// Brings a tensor map (a __grid_constant__ parameter) into the descriptor cache ahead of the first copy that uses it.
+__device__ __forceinline__ void prefetch_map(const void* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // global -> shared bulk copy; completion (byte count) is signalled on `bar`.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"

@@ -132,6 +132,8 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
     float* merge = reinterpret_cast<float*>(smem_d + (ring - smem_u32(smem_d)) + kDecStages * 2 * kTileBytes);
 
     if (threadIdx.x == 0) {
+        prefetch_map(&kmap);
+        prefetch_map(&vmap);
         for (int s = 0; s < kDecStages; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_empty[s], kDecWarps); }
         mbar_init_fence();
     }

@@ -353,6 +353,9 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     const int lane = threadIdx.x & 31, warp = static_cast<int>(warp_uniform(threadIdx.x >> 5));
     const uint32_t q_smem = (smem_u32(smem_p) + 1023u) & ~1023u, ring = q_smem + 2 * Shape::kTileBytes;
     if (threadIdx.x == 0) {
+        prefetch_map(&qmap);
+        prefetch_map(&kmap);
+        prefetch_map(&vmap);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.item_full[i], 1);
             mbar_init(&bar.item_empty[i], 13);                     // warps 0-12
