@@ -309,13 +309,19 @@ int nmt_sdpa_decode_paged_bf16(const nmt_paged_cache* cache, const void* q, int6
  *   q, out bf16 [q_tokens][heads][head_dim], k, v bf16 [kv_tokens][kv_heads][head_dim], any token and head strides
  *              (elements, multiples of 8): a view of a joint projection's output, or of the caches of
  *              nmt_sdpa_decode_bf16.  head_dim 64 or 128, heads a multiple of kv_heads, scale positive and finite.
- * fp32 scores, statistics and sums; the weights are rounded to bf16 once for the product with v.  What a mask hides is
- * never used, not even an infinity or a NaN in v.  No workspace.  One launch. */
+ * fp32 scores, statistics and sums; the weights are good to 2^-18 and rounded to bf16 once for the product with v.  What a
+ * mask hides is never used, not even an infinity or a NaN in v.
+ *   workspace  nmt_sdpa_prefill_workspace_bytes(...) bytes, 32-byte aligned, no initialisation; calls whose kernels may
+ *              overlap need one each.  The size is 0 unless the keys of few queries may be worth cutting into pieces, one
+ *              per SM (a few new tokens over a long prefix); NULL is always allowed and cuts nothing.
+ * The work is cut by the lengths alone, so results repeat bit for bit.  One launch, two with a workspace that is used. */
+int64_t nmt_sdpa_prefill_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim);
 int nmt_sdpa_prefill_bf16(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
                           int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, void* out,
                           int64_t out_token_stride, int64_t out_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch,
                           int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
-                          void* stream);
+                          void* workspace, void* stream);
 
 /* fp32 twin, unsplit; replaces causal_conv1d_prefill_fp32 (ops/mamba2/causal_conv1d.cuh:115-127). */
 int nmt_causal_conv1d_silu_f32(const float* x, const float* w, const float* bias, float* y, float* state_out,

@@ -53,8 +53,9 @@ PROTOTYPES = {
                                         _p, _p]),
     "nmt_sdpa_decode_paged_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "nmt_sdpa_decode_paged_bf16": (_int, [_cache, _p, _i64, _i64, _p, _i64, _i64, _i64, _f, _p, _p, _p]),
+    "nmt_sdpa_prefill_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "nmt_sdpa_prefill_bf16": (_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f,
-                                     _int, _p]),
+                                     _int, _p, _p]),
     "nmt_ssm_decode_step_bf16": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f, _f, _p]),
     "nmt_relu2_f32": (_int, [_p, _p, _i64, _p]),
     "nmt_add_bf16": (_int, [_p, _p, _p, _i64, _p]),

@@ -31,6 +31,12 @@ constexpr int kPfTile = 128;                                       // rows of a 
 constexpr int kSoftmaxRegs = 200, kEpilogueRegs = 56, kOtherRegs = 56;    // 2 x 200 + 56 + 56 = 512 = 4 x the launch's 128
 constexpr float kLag = 8.f;                                        // log2 of how far M may lag
 
+// Cutting an item's keys into pieces, when there are fewer items than SMs' worth of work (a few new queries over a long prefix).
+constexpr int kPfMinPiece = 8;                                     // K / V tiles of a piece, at least
+constexpr int kPfSlack = 4;                                        // an item this much over the average is left whole
+constexpr int kPfPieces = 2 * kSmCount;                            // pieces there can be (see pieces())
+constexpr int kPfSplitItems = 4 * kSmCount;                        // with more items than this nothing is cut
+
 template <int D>
 struct PfShape {
     static constexpr int kTileBytes = kPfTile * D * 2;             // Q tile, K tile or V tile
@@ -41,6 +47,8 @@ struct PfShape {
 
 struct PrefillArgs {
     __nv_bfloat16* out;
+    float* part_o;                                 // pieces: [kPfPieces][2][128][D] sums of weights times values; NULL: nothing is cut
+    float2* part_ml;                               // [kPfPieces][2][128]: maximum (log 2 units) and sum of the weights
     const __nv_bfloat16 *q, *k, *v;
     const int32_t *cu_q, *cu_k;
     int64_t o_ts, o_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
@@ -54,6 +62,8 @@ struct PfItem {
     // per query tile: first row in q and out, valid rows (1 .. 128), keys that row 0 sees before clamping (row r sees limit + r
     // when causal), head, K / V tiles.  n[0] < 0: no more items; n[1] == 0: one query tile only.  n[0] <= n[1] otherwise.
     int q_row[2], rows[2], limit[2], head[2], n[2];
+    int first;                                     // first K / V tile: 0 unless this is a piece of a cut item
+    int slot;                                      // where a piece leaves its result; < 0: a whole item, written to out
 };
 
 // Shared-memory matrix descriptors, as two words so that a step along an operand is one 32-bit addition.  High word: 1024
@@ -208,40 +218,87 @@ struct PfSequence {
         const int block = short_of < 0 ? 0 : min(short_of / kPfTile, (n - 1) / kPfTile);
         return all - block * p.group / 2;                          // items whose second tile is in that block or a later one
     }
+    // K / V tiles of the longest item, and of the shortest.
+    __device__ __forceinline__ int longest() const { return n > 0 ? max(1, (m + kPfTile - 1) / kPfTile) : 0; }
+    __device__ __forceinline__ int shortest(const PrefillArgs& p) const {
+        if (!p.causal || n == 0) return longest();
+        const int block = p.group == 1 && n > kPfTile ? 1 : 0;     // of the first item's second query tile
+        return max(1, (min(m, m - n + min(n, (block + 1) * kPfTile)) + kPfTile - 1) / kPfTile);
+    }
+    // K / V tiles of all items together: the sum over c of items_from(c).
+    __device__ __forceinline__ int64_t work(const PrefillArgs& p) const {
+        const int64_t all = items(p), most = (m + kPfTile - 1) / kPfTile;
+        if (!p.causal || most <= 1) return all * max(most, (int64_t)1);
+        // items_from(c) = all - floor(k G / 2) with k = max(c - 1 - e, 0), e = ceil((m - n) / 128), for c = 2 .. most
+        const int64_t e = m >= n ? (m - n + kPfTile - 1) / kPfTile : -((n - m) / kPfTile), g = p.group;
+        auto sum = [&](int64_t x) {                                // of floor(k G / 2), k = 0 .. x
+            return x <= 0 ? (int64_t)0 : (g * (x * (x + 1) / 2) - ((g & 1) ? (x + 1) / 2 : 0)) / 2;
+        };
+        return all * most - (sum(most - 1 - e) - sum(e < 0 ? -e : 0));
+    }
 };
 struct PfOrder {
-    int cost, base, count, chunk, before;          // cost now handed out, items of higher cost, of this one; place among the sequences
+    int cost, base, count, chunk, before;          // cost now handed out, pieces of higher cost, items of this one; place among the sequences
+    int below;                                     // the next lower cost that some item has
+    int share;                                     // K / V tiles that would be every SM's equal part, or more than any item has
+
+    // Pieces of an item with c K / V tiles.  Only items of more than `share` are cut, into fewer than 2 c / share pieces, and all
+    // items together have at most share * kSmCount tiles: at most kPfPieces pieces, the first in the order.
+    __device__ __forceinline__ int pieces(int c) const { return c <= share + kPfSlack ? 1 : (c + share - 1) / share; }
 
     __device__ __forceinline__ void seat(const PrefillArgs& p, int c) {
         cost = c;
         chunk = before = 0;
-        int mine = 0;
+        int mine = 0, next = 0;
         if (cost > 0)
             for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
                 const PfSequence q(p, b);
                 mine += q.items_from(p, cost) - q.items_from(p, cost + 1);
+                const int lower = min(cost - 1, q.longest());
+                if (lower >= q.shortest(p)) next = max(next, lower);
             }
         count = __reduce_add_sync(0xffffffffu, mine);
+        below = __reduce_max_sync(0xffffffffu, next);
     }
     __device__ __forceinline__ void start(const PrefillArgs& p) {
         int most = 0;
+        int64_t all = 0;
         for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
             const PfSequence q(p, b);
-            if (q.n > 0) most = max(most, max(1, (q.m + kPfTile - 1) / kPfTile));
+            most = max(most, q.longest());
+            all += q.work(p);
+        }
+        share = 0x3fffffff;
+        if (p.part_o) {
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+            share = static_cast<int>(min(max((all * p.kv_heads + kSmCount - 1) / kSmCount, (int64_t)kPfMinPiece), (int64_t)0x3fffffff));
         }
         base = 0;
         seat(p, __reduce_max_sync(0xffffffffu, most));
     }
-    // False: there is no such item.
+    __device__ __forceinline__ int piece_len() const { return (cost + pieces(cost) - 1) / pieces(cost); }
+    // The which-th item that is cut, as its first piece.  False: there is no such item.
+    __device__ __forceinline__ bool find_cut(const PrefillArgs& p, int which, PfItem& it) {
+        int items = 0;                                             // of higher cost
+        while (cost > 0 && pieces(cost) > 1 && which >= items + count * p.kv_heads) {
+            items += count * p.kv_heads;
+            base += count * p.kv_heads * pieces(cost);
+            seat(p, below);
+        }
+        return cost > 0 && pieces(cost) > 1 && find(p, base + (which - items) * pieces(cost), it);
+    }
+    // The piece or item with this number.  False: there is none.
     __device__ __forceinline__ bool find(const PrefillArgs& p, int index, PfItem& it) {
         const int lane = threadIdx.x & 31;
-        while (cost > 0 && index >= base + count * p.kv_heads) {
-            base += count * p.kv_heads;
-            seat(p, cost - 1);
+        while (cost > 0 && index >= base + count * p.kv_heads * pieces(cost)) {
+            base += count * p.kv_heads * pieces(cost);
+            seat(p, below);
         }
         if (cost <= 0) return false;
-        const int rank = (index - base) / p.kv_heads;
-        it.kv_head = (index - base) % p.kv_heads;
+        const int cut = pieces(cost), piece = (index - base) % cut, which = (index - base) / cut;
+        const int rank = which / p.kv_heads;
+        it.kv_head = which % p.kv_heads;
         // the sequence whose share of this cost holds `rank`
         int mine, upto;
         for (;;) {
@@ -278,6 +335,12 @@ struct PfOrder {
             const int sees = p.causal ? min(q.m, it.limit[t] + it.rows[t] - 1) : q.m;
             it.n[t] = 2 * item + t < tiles ? max(1, (sees + kPfTile - 1) / kPfTile) : 0;
         }
+        const int len = piece_len();
+        it.first = piece * len;
+        it.slot = cut > 1 ? index : -1;
+        if (cut > 1)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) it.n[t] = min(max(it.n[t] - it.first, 0), len);
         return holds != 0;
     }
 };
@@ -419,7 +482,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tm_ld32(reinterpret_cast<uint32_t*>(s) + 32 * c, s_addr + 32 * c);
                 tm_wait_ld();
-                const int left = sees - j * kPfTile;
+                const int left = sees - (it.first + j) * kPfTile;
                 const bool masked = __any_sync(0xffffffffu, left < kPfTile);
                 if (masked) {
 #pragma unroll
@@ -461,6 +524,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
             if (o_uses > 0 && !warp_wait(&bar.o_empty[t], (o_uses - 1) & 1u)) break;    // the last item's L has been read
             ++o_uses;
             s_l[t][wq * 32 + lane] = l2.x + l2.y;
+            if (it.slot >= 0) p.part_ml[((size_t)it.slot * 2 + t) * kPfTile + wq * 32 + lane] = make_float2(m * p.scale_log2, l2.x + l2.y);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.l_full[t]);
         }
@@ -488,6 +552,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 __nv_bfloat16* dst = p.out + (int64_t)(it.q_row[t] + r) * p.o_ts + (int64_t)it.head[t] * p.o_hs;
                 const uint32_t o_addr = tmem + lanes + 256 + t * kPfTile;
                 float2 odd2 = make_float2(0.f, 0.f);               // 0 x (a value that is not finite) is NaN
+                float* part = p.part_o + (((size_t)max(it.slot, 0) * 2 + t) * kPfTile + r) * D;
                 uint32_t o[2][16];
                 tm_ld16(o[0], o_addr);
 #pragma unroll
@@ -499,6 +564,13 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         tm_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&bar.o_empty[t]);
+                    }
+                    if (it.slot >= 0) {                            // a piece: as it is, for the join
+                        if (r < it.rows[t]) {
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(part + 16 * c), NMT_W8(o[c & 1], 0) : "memory");
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(part + 16 * c + 8), NMT_W8(o[c & 1], 8) : "memory");
+                        }
+                        continue;
                     }
                     uint32_t w[8];
 #pragma unroll
@@ -516,7 +588,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         }
                     }
                 }
-                const bool odd = !none && r < it.rows[t] && odd2.x + odd2.y != 0.f;
+                const bool odd = !none && r < it.rows[t] && it.slot < 0 && odd2.x + odd2.y != 0.f;
                 for (uint32_t redo = __ballot_sync(0xffffffffu, odd && l < INFINITY); redo; redo &= redo - 1) {
                     const int rr = wq * 32 + __ffs(redo) - 1;
                     redo_row<D>(p, it.q_row[t] + rr, it.head[t], it.kv_row, p.causal ? min(it.kv_len, it.limit[t] + rr) : it.kv_len);
@@ -658,11 +730,11 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     if (kv >= ST) ok = warp_wait(&bar.kv_empty[st], (kv / ST - 1) & 1u);
                     if (!ok) break;
                     const uint32_t dst = ring + st * Shape::kTileBytes;
-                    const int valid = it.kv_len - (i >> 1) * kPfTile;
+                    const int tile = it.first + (i >> 1), valid = it.kv_len - tile * kPfTile;
                     if ((i & 1) && valid < kPfTile) {
                         // Keys past the sequence's end belong to another one or to nobody, and 0 x NaN is NaN: their rows of V
                         // are cleared before anybody is told that the tile is there.
-                        load(&vmap, it.kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.v_raw);
+                        load(&vmap, it.kv_head, it.kv_row + tile * kPfTile, dst, &bar.v_raw);
                         ok = warp_wait(&bar.v_raw, v_raws++ & 1u);
                         if (!ok) break;
                         const int from = max(valid, 0);
@@ -675,7 +747,7 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                         if (lane == 0) mbar_arrive(&bar.kv_full[st]);
                         __syncwarp();
                     } else {
-                        load(i & 1 ? &vmap : &kmap, it.kv_head, it.kv_row + (i >> 1) * kPfTile, dst, &bar.kv_full[st]);
+                        load(i & 1 ? &vmap : &kmap, it.kv_head, it.kv_row + tile * kPfTile, dst, &bar.kv_full[st]);
                     }
                     if (i == 0) load_q(1);
                 }
@@ -699,40 +771,135 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     pdl_trigger();
 }
 
+// Joins the pieces of the items that were cut: CTA (i, t, quarter) takes 32 rows of query tile t of the i-th such item; a warp
+// takes a row at a time, a lane D / 32 columns.  The order of items is worked out again, which is shorter than passing it
+// on would be.
+constexpr int kPfJoinWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kPfJoinWarps * 32)
+sdpa_prefill_join_kernel(const PrefillArgs p) {
+    constexpr int W = D / 64;
+    __shared__ PfItem s_it;
+    __shared__ int s_cut, s_len;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.y;
+    pdl_wait();
+    if (warp == 0) {
+        PfOrder order;
+        PfItem it;
+        order.start(p);
+        const bool have = order.find_cut(p, blockIdx.x, it);
+        if (lane == 0) {
+            s_cut = have ? order.pieces(order.cost) : 0;
+            s_len = have ? order.piece_len() : 0;
+            s_it = it;
+        }
+    }
+    __syncthreads();
+    const PfItem& it = s_it;
+    const int cut = s_cut, len = s_len;
+    if (cut > 0 && it.n[t] > 0) {
+        for (int r = blockIdx.z * 32 + warp; r < min(it.rows[t], static_cast<int>(blockIdx.z) * 32 + 32); r += kPfJoinWarps) {
+            const int sees = p.causal ? min(it.kv_len, it.limit[t] + r) : it.kv_len;
+            // pieces past the last key that the row sees hold nothing of it (and may not have looked at this tile at all)
+            const int n = min(cut, max(1, (sees + len * kPfTile - 1) / (len * kPfTile)));
+            auto at = [&](int i) { return ((size_t)(it.slot + i) * 2 + t) * kPfTile + r; };
+            float top = -INFINITY;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_ml[at(i)].x);
+            float sum = 0.f;
+            float2 acc[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) acc[e] = make_float2(0.f, 0.f);
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const float2 ml = p.part_ml[at(i)];
+                if (ml.y == 0.f) continue;                         // sees nothing there: whatever its products hold
+                const float w = pf_ex2(ml.x - (top == -INFINITY ? 0.f : top));
+                sum = fmaf(w, ml.y, sum);
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    const float2 o = *reinterpret_cast<const float2*>(p.part_o + at(i) * D + e * 64 + lane * 2);
+                    acc[e].x = fmaf(w, o.x, acc[e].x);
+                    acc[e].y = fmaf(w, o.y, acc[e].y);
+                }
+            }
+            const bool none = sees <= 0 || sum == 0.f;
+            bool odd = false;
+            __nv_bfloat16* dst = p.out + (int64_t)(it.q_row[t] + r) * p.o_ts + (int64_t)it.head[t] * p.o_hs;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                const float x = none ? 0.f : acc[e].x / sum, y = none ? 0.f : acc[e].y / sum;
+                odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+                *reinterpret_cast<uint32_t*>(dst + e * 64 + lane * 2) = pack_bf16x2(x, y);
+            }
+            if (__any_sync(0xffffffffu, odd) && sum < INFINITY) redo_row<D>(p, it.q_row[t] + r, it.head[t], it.kv_row, sees);
+        }
+    }
+    pdl_trigger();
+}
+
 template <int D>
 static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, int items, cudaStream_t st) {
     auto kern = sdpa_prefill_kernel<D>;
     static std::atomic<uint64_t> allowed{0};
     allow_smem(kern, PfShape<D>::kSmem, allowed);
-    launch_kernel(kern, items, kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
+    launch_kernel(kern, items + (p.part_o ? kPfPieces : 0), kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
+    if (p.part_o) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(kSmCount, 2, kPfTile / 32);             // a cut item has more than an SM's equal part: fewer than kSmCount of them
+        cfg.blockDim = dim3(kPfJoinWarps * 32);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 1 : 0;
+        cudaLaunchKernelEx(&cfg, sdpa_prefill_join_kernel<D>, p);
+    }
+}
+
+// Items: two query tiles (128 rows of a head) of a sequence and kv head each.  As many as the batch can have (every sequence
+// may end in a partly filled block and an odd tile); CTAs past the real number find nothing to do.
+static int64_t prefill_items(int64_t batch, int64_t q_tokens, int64_t heads, int64_t kv_heads) {
+    const int64_t full = (q_tokens + kPfTile - 1) / kPfTile, blocks = q_tokens < full + batch - 1 ? q_tokens : full + batch - 1;
+    return (blocks * (heads / kv_heads) + (blocks < batch ? blocks : batch)) / 2 * kv_heads;
+}
+// Whether some item can be worth cutting, from what the host knows: few items, and keys for at least two pieces.  One
+// sequence is known well enough to tell that its longest item is no more than an SM's equal part.
+static bool prefill_may_cut(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads) {
+    const int64_t most = (kv_tokens + kPfTile - 1) / kPfTile, items = prefill_items(batch, q_tokens, heads, kv_heads);
+    if (items > kPfSplitItems || most <= kPfMinPiece + kPfSlack) return false;
+    return batch > 1 || (most - kPfSlack) * kSmCount > items * (2 * kv_tokens - q_tokens) / (2 * kPfTile);
 }
 
 }  // namespace nmt
 
 extern "C" {
 
+int64_t nmt_sdpa_prefill_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+    using namespace nmt;
+    if (batch <= 0 || q_tokens <= 0 || kv_tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads) return 0;
+    return prefill_may_cut(batch, q_tokens, kv_tokens, heads, kv_heads) ? (int64_t)kPfPieces * 2 * kPfTile * (head_dim * 4 + 8) : 0;
+}
+
 int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
                           int64_t v_hs, void* out, int64_t o_ts, int64_t o_hs, const int32_t* cu_q, const int32_t* cu_k, int64_t batch,
                           int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
-                          void* stream) {
+                          void* workspace, void* stream) {
     using namespace nmt;
     if (batch < 0 || q_tokens < 0 || kv_tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || !(scale > 0.f) || !(scale < INFINITY))
         return NMT_ERR_SHAPE;
     if ((!cu_q && (batch != 1 || cu_k))) return NMT_ERR_SHAPE;
     if (head_dim != 64 && head_dim != 128) return NMT_ERR_UNSUPPORTED;
     if (q_tokens > 0x3fffffff || kv_tokens > 0x3fffffff || batch > 0x3fffffff || heads > 65535) return NMT_ERR_UNSUPPORTED;
-    // Items: two query tiles (128 rows of a head) of a sequence and kv head each.  As many as the batch can have (every
-    // sequence may end in a partly filled block and an odd tile); CTAs past the real number find nothing to do.
-    const int64_t full = (q_tokens + kPfTile - 1) / kPfTile, some = cu_q ? batch : 1;
-    const int64_t blocks = q_tokens < full + some - 1 ? q_tokens : full + some - 1, group = heads / kv_heads;
-    const int64_t items = (blocks * group + (blocks < some ? blocks : some)) / 2 * kv_heads;
-    if (blocks * heads > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
+    const int64_t items = prefill_items(batch, q_tokens, heads, kv_heads);
+    if (items > 0x3fffffff) return NMT_ERR_UNSUPPORTED;
     if (q_tokens == 0 || batch == 0) return NMT_OK;
     int st;
     if ((st = check_view(q, q_tokens, q_ts, heads, q_hs)) != NMT_OK || (st = check_view(out, q_tokens, o_ts, heads, o_hs)) != NMT_OK) return st;
     if (kv_tokens > 0 && ((st = check_view(k, kv_tokens, k_ts, kv_heads, k_hs)) != NMT_OK || (st = check_view(v, kv_tokens, v_ts, kv_heads, v_hs)) != NMT_OK))
         return st;
-    if (!aligned4(cu_q) || !aligned4(cu_k)) return NMT_ERR_ALIGN;
+    if (!aligned4(cu_q) || !aligned4(cu_k) || (reinterpret_cast<uintptr_t>(workspace) & 31u)) return NMT_ERR_ALIGN;
     EncodeTiledFn encode = encode_tiled_fn();
     if (!encode) return NMT_ERR_UNSUPPORTED;
     // Without keys there is nothing to describe (and nothing that is read counts): any valid row will do.
@@ -761,10 +928,13 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
     p.batch = static_cast<int>(batch); p.q_tokens = static_cast<int>(q_tokens); p.kv_tokens = static_cast<int>(kv_tokens);
     p.kv_heads = static_cast<int>(kv_heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
     p.out32 = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && (q_tokens == 1 || o_ts % 16 == 0) && (heads == 1 || o_hs % 16 == 0);
+    const bool cut = workspace && prefill_may_cut(batch, q_tokens, kv_tokens, heads, kv_heads);
+    p.part_o = cut ? static_cast<float*>(workspace) : nullptr;
+    p.part_ml = cut ? reinterpret_cast<float2*>(p.part_o + (size_t)kPfPieces * 2 * kPfTile * head_dim) : nullptr;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, static_cast<int>(items), cs);
     else launch_prefill<64>(maps[0], maps[1], maps[2], p, static_cast<int>(items), cs);
-    return finish_launch(1);
+    return finish_launch(cut ? 2 : 1);
 }
 
 }  // extern "C"

@@ -437,16 +437,22 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
+def sdpa_prefill_workspace(batch: int, tokens: int, kv_tokens: int, heads: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Workspace of sdpa_prefill for these sizes (often empty); calls that may overlap on the GPU need one each."""
+    return torch.empty(_lib.load().nmt_sdpa_prefill_workspace_bytes(batch, tokens, kv_tokens, heads, kv_heads, head_dim), dtype=torch.uint8,
+                       device=device)
+
+
 @_on_device
 def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
                  cu_seqlens_k: torch.Tensor | None = None, causal: bool = True, scale: float | None = None,
-                 out: torch.Tensor | None = None) -> torch.Tensor:
+                 out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of whole prompts, packed one after the other: q [tokens, heads, head_dim], k / v [kv_tokens, kv_heads,
     head_dim], bf16 views with any token and head strides.  cu_seqlens int32 [batch + 1] (device) cuts the rows of q, and of
     k and v unless cu_seqlens_k cuts those; None is one sequence of all rows.  With causal, query i of a sequence of n
     queries and m keys sees keys j <= i + (m - n): a sequence whose first part is cached passes more keys than queries.  A
     query that sees nothing gives zeros.  Rows behind the last sequence are not written.  scale defaults to
-    1 / sqrt(head_dim)."""
+    1 / sqrt(head_dim).  workspace: sdpa_prefill_workspace(...), which is empty for most sizes; allocated here if not given."""
     dev = q.device
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q, k and v must be bf16 [tokens, heads, head_dim]")
@@ -468,9 +474,16 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: 
         raise ValueError("cu_seqlens_k without cu_seqlens")
     out = q.new_empty(q.shape) if out is None else out
     os = _result3(out, "out", T, heads, dim, dev)
-    _lib.check(_lib.load().nmt_sdpa_prefill_bf16(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                                                 out.data_ptr(), os[0], os[1], cu, cu_k, batch, T, T_k, heads, kv_heads, dim,
-                                                 dim ** -0.5 if scale is None else scale, 1 if causal else 0, _raw_stream(dev.index)), "sdpa_prefill")
+    lib = _lib.load()
+    need = lib.nmt_sdpa_prefill_workspace_bytes(batch, T, T_k, heads, kv_heads, dim)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif need and (workspace.device != dev or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need):
+        raise ValueError("workspace too small, not contiguous or on another device")
+    _lib.check(lib.nmt_sdpa_prefill_bf16(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                         out.data_ptr(), os[0], os[1], cu, cu_k, batch, T, T_k, heads, kv_heads, dim,
+                                         dim ** -0.5 if scale is None else scale, 1 if causal else 0,
+                                         workspace.data_ptr() if need else None, _raw_stream(dev.index)), "sdpa_prefill")
     return out
 
 

@@ -127,8 +127,8 @@ def test_rope_table_is_exact_at_far_positions():
         assert abs(t[pos, i].item() - math.cos(a)) <= 2.0 ** -24 + 1e-9 and abs(t[pos, 32 + i].item() - math.sin(a)) <= 2.0 ** -24 + 1e-9
 
 
-def prefill(L, q=BUF, qts=5120, k=BUF, kts=1024, v=BUF, out=BUF, cu=BUF, cu_k=None, batch=2, T=5, T_k=5, heads=40, kv=8, dim=128, scale=0.1):
-    return L.nmt_sdpa_prefill_bf16(q, qts, 128, k, kts, 128, v, 1024, 128, out, 5120, 128, cu, cu_k, batch, T, T_k, heads, kv, dim, scale, 1, None)
+def prefill(L, q=BUF, qts=5120, k=BUF, kts=1024, v=BUF, out=BUF, cu=BUF, cu_k=None, batch=2, T=5, T_k=5, heads=40, kv=8, dim=128, scale=0.1, ws=None):
+    return L.nmt_sdpa_prefill_bf16(q, qts, 128, k, kts, 128, v, 1024, 128, out, 5120, 128, cu, cu_k, batch, T, T_k, heads, kv, dim, scale, 1, ws, None)
 
 
 def test_prefill(built_lib):
@@ -145,6 +145,9 @@ def test_prefill(built_lib):
     for name in ("q", "k", "v", "out"):
         assert prefill(L, **{name: None}) == NULL and prefill(L, **{name: BUF + 8}) == ALIGN
     assert prefill(L, qts=5124) == ALIGN and prefill(L, kts=-1024) == UNSUPPORTED
-    assert prefill(L, cu=BUF + 2) == ALIGN
+    assert prefill(L, cu=BUF + 2) == ALIGN and prefill(L, ws=BUF + 16) == ALIGN
+    size = L.nmt_sdpa_prefill_workspace_bytes
+    assert size(1, 16384, 16384, 40, 8, 128) == 0 and size(1, 200, 200, 40, 8, 128) == 0 and size(4, 100, 1000, 40, 7, 128) == 0
+    assert size(4, 100, 20000, 40, 8, 128) > 0 and size(1, 1, 20000, 40, 8, 64) > 0
     assert prefill(L, T=1 << 31, T_k=1 << 31) == UNSUPPORTED
     assert L.nmt_launch_count() == before

@@ -72,6 +72,37 @@ def test_against_the_formula(ops, ns, ms, heads, kv_heads, dim, causal, peak):
         assert torch.equal(ops.sdpa_prefill(q, k, v, causal=causal).view(torch.int16), out.view(torch.int16))
 
 
+@pytest.mark.parametrize("ns,ms,heads,kv_heads,dim,causal", [
+    ([1], [5000], 10, 2, 128, True),
+    ([3, 1000, 8], [9000, 1500, 2], 8, 2, 64, True),
+    ([129, 1, 1, 300], [3000, 6001, 128, 300], 5, 1, 128, True),
+    ([200], [20000], 4, 4, 64, False),
+    ([700, 4], [300, 4000], 4, 2, 128, True),                         # queries that see nothing beside a long prefix
+    ([257], [7777], 2, 1, 128, True),
+])
+@pytest.mark.parametrize("peak", [1.0, 6.0])
+def test_few_queries_over_long_prefixes(ops, ns, ms, heads, kv_heads, dim, causal, peak):
+    """The keys of an item cut into pieces: with the workspace, without one, and with values behind the mask that are not finite."""
+    g = gen(sum(ms) + heads)
+    q = (peak * randn(g, sum(ns), heads, dim)).to(BF)
+    k, v = randn(g, sum(ms), kv_heads, dim).to(BF), randn(g, sum(ms), kv_heads, dim).to(BF)
+    ws = ops.sdpa_prefill_workspace(len(ns), sum(ns), sum(ms), heads, kv_heads, dim)
+    assert ws.numel() > 0
+    ws.fill_(255)                                                    # NaN everywhere: nothing of it may be used
+    args = (q, k, v, cu_of(ns), cu_of(ms))
+    out = ops.sdpa_prefill(*args, causal=causal, workspace=ws)
+    compare(out, q, k, v, ns, ms, causal, dim ** -0.5, rows=300)
+    assert torch.equal(out.view(torch.int16), ops.sdpa_prefill(*args, causal=causal).view(torch.int16)), "the same call gave other bits"
+    if causal and ns[0] > 1 and ms[0] > ns[0]:
+        at = ms[0] - ns[0] // 2
+        v2 = v.clone()
+        v2[at] = math.nan
+        hit = ops.sdpa_prefill(q, k, v2, cu_of(ns), cu_of(ms), workspace=ws)
+        first = ns[0] - (ms[0] - at)                                 # the first query that sees key `at`
+        compare(hit[:first], q, k, v, [first], [first + ms[0] - ns[0]], True, dim ** -0.5, rows=300)
+        assert bool(hit[first:ns[0]].isnan().all())
+
+
 def test_long_prompt(ops):
     g = gen(3)
     n = 20011
