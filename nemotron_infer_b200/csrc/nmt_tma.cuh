@@ -75,8 +75,8 @@ __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity) {
 }
 
 // The same wait without a suspension hint: a waiter is woken as soon as the phase completes, which the hinted form above does
-// not promise (a ping-pong of waits of a few hundred cycles each ran at less than half its speed with it).  Bounded by the
-// clock: about two seconds, looked at every 256 polls.
+// not promise (prompt attention, whose warps hand work back and forth every few hundred cycles, took 3.04 ms instead of 2.15
+// with it).  Bounded by the clock: about two seconds, looked at every 256 polls.
 __device__ __forceinline__ bool mbar_try_wait_now(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(

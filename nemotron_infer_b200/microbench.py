@@ -47,6 +47,10 @@ SHAPES = {
     "gemv_o": (3136, 5120),          # attention o_proj N = 3136, K = 5120 (q / k / v: --op gemv_up --tokens 5120 / 1024)
     "ssm_step": (1, 2 * 96 * 80 * 128 * 4),   # per sequence: the fp32 state [96, 80, 128] read and written once
     "sdpa_decode": (512, 2 * 8 * 128 * 2),    # per cached token: one K and one V row of each of the 8 KV heads
+    # attention over a paged cache and over whole prompts, 40 query / 8 KV heads of 128
+    "kv_append_paged": (4096, ((2 * 8 + 40) * 2 * 128) * 2 + 128 * 4),   # per token: K, V, Q in, cache rows and rotated Q out, one rotation row
+    "sdpa_decode_paged": (2048, 32 * 2 * 8 * 128 * 2),          # per cached token of each of 32 sequences
+    "sdpa_prefill": (8192, (2 * 40 + 2 * 8) * 128 * 2),         # one causal prompt; bound by its 4 * 128 * 40 * T^2 / 2 flops (see "tflops")
     # e4m3 activation quantisation (the step after the norm / activation in the FP8 blocks)
     "quantize_fp8": (8192, 3136 * (2 + 2 + 1)),                  # amax pass + quantising pass over [T, 3136]
     "add_rmsnorm_quant_fp8": (8192, 3136 * (2 + 2 + 2 + 2 + 1)),  # x, r -> out_res ; out_res -> e4m3
@@ -99,6 +103,25 @@ def make_case(op: str, T: int, dev):
         o = torch.empty(H_Q, 128, dtype=BF, device=dev)
         ws = torch.empty(max(16, _lib.load().nmt_sdpa_decode_workspace_bytes(T, H_Q)), dtype=torch.uint8, device=dev)
         return lambda: ops.sdpa_decode(q, k, v, kn, vn, T, out=o, workspace=ws)
+    if op in ("kv_append_paged", "sdpa_decode_paged"):
+        H_Q, H_KV, page, B = 40, 8, 64, 1 if op == "kv_append_paged" else 32
+        per = -(-T // page)
+        k, v = rn(B * per, H_KV, page, 128).to(BF), rn(B * per, H_KV, page, 128).to(BF)
+        table = torch.randperm(B * per, device=dev).to(torch.int32).view(B, per)
+        lens = torch.full((B,), T, dtype=torch.int32, device=dev)
+        if op == "sdpa_decode_paged":
+            q = rn(B, H_Q, 128).to(BF)
+            o, ws = torch.empty_like(q), ops.sdpa_decode_paged_workspace(B, H_Q, H_KV, 128, dev)
+            return lambda: ops.sdpa_decode_paged(q, k, v, table, lens, out=o, workspace=ws)
+        x = rn(T, H_Q + 2 * H_KV, 128).to(BF)
+        cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+        rope = ops.rope_table(T, 128, device=dev)
+        o = torch.empty(T, H_Q, 128, dtype=BF, device=dev)
+        return lambda: ops.kv_append_paged(x[:, H_Q:H_Q + H_KV], x[:, H_Q + H_KV:], k, v, table, lens, cu, q=x[:, :H_Q], rope=rope, q_out=o)
+    if op == "sdpa_prefill":
+        q, k, v = rn(T, 40, 128).to(BF), rn(T, 8, 128).to(BF), rn(T, 8, 128).to(BF)
+        o = torch.empty_like(q)
+        return lambda: ops.sdpa_prefill(q, k, v, out=o)
     if op == "ssm_step":
         H, P, N, G = 96, 80, 128, 8
         x, dt = rn(T, H * P).to(BF), (rn(T, H) - 1).to(BF)
@@ -180,7 +203,8 @@ def run_op(op: str, T: int, reps: int, warmup: int, dev, batch: int = 10, graph:
     med, mn = statistics.median(us), us[0]
     peak = measured_peak()
     gbs = nbytes / med / 1e3
-    return {"op": op, "tokens": T, "bytes_per_token": bpt, "buffer_sets": nsets, "reps": reps, "batch": batch, "graph": graph,
+    extra = {"tflops": round(2 * 128 * 40 * T * (T + 1) / med / 1e6, 1)} if op == "sdpa_prefill" else {}
+    return {**extra, "op": op, "tokens": T, "bytes_per_token": bpt, "buffer_sets": nsets, "reps": reps, "batch": batch, "graph": graph,
             "median_us": round(med, 2), "min_us": round(mn, 2), "gbs": round(gbs, 1),
             "gbs_best": round(nbytes / mn / 1e3, 1), "tokens_per_s": round(T / med * 1e6, 0),
             "frac_of_nominal_8000": round(gbs / NOMINAL_GBS, 4),
@@ -254,7 +278,7 @@ def main() -> None:
             print(json.dumps(run_fixed_cost(op, T, a.reps, f"cuda:{a.device}")), flush=True)
             torch.cuda.empty_cache()
             continue
-        print(json.dumps(run_op(op, T, a.reps, a.warmup, f"cuda:{a.device}", a.batch, a.graph or op.startswith("gemv") or op in ("ssm_step", "sdpa_decode"))), flush=True)
+        print(json.dumps(run_op(op, T, a.reps, a.warmup, f"cuda:{a.device}", a.batch, a.graph or op.startswith("gemv") or op in ("ssm_step", "sdpa_decode", "kv_append_paged", "sdpa_decode_paged", "sdpa_prefill"))), flush=True)
         torch.cuda.empty_cache()
 
 
