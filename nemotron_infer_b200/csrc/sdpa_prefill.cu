@@ -537,61 +537,72 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         PfItem it;
         bool ok = true;
         for (int k = 0; ok && next_item(k, it); ++k) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (it.n[t] == 0 || !ok) continue;
-                ok = warp_wait(&bar.l_full[t], uses[t] & 1u) && warp_wait(&bar.o_full[t], uses[t] & 1u);
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {                          // loops that are not unrolled: short items are bound by the instructions they run through once
+                if ((t == 0 ? it.n[0] : it.n[1]) == 0 || !ok) continue;
+                const uint32_t phase = (t == 0 ? uses[0]++ : uses[1]++) & 1u;
+                ok = warp_wait(&bar.l_full[t], phase) && warp_wait(&bar.o_full[t], phase);
                 if (!ok) continue;
-                ++uses[t];
                 tm_fence_after();
-                const int r = wq * 32 + lane;
+                const int r = wq * 32 + lane, q_row = t == 0 ? it.q_row[0] : it.q_row[1], head = t == 0 ? it.head[0] : it.head[1];
+                const int limit = t == 0 ? it.limit[0] : it.limit[1];
+                const bool valid = r < (t == 0 ? it.rows[0] : it.rows[1]);
                 const float l = s_l[t][r];
-                const int sees = p.causal ? min(it.kv_len, it.limit[t] + r) : it.kv_len;
+                const int sees = p.causal ? min(it.kv_len, limit + r) : it.kv_len;
                 const bool none = sees <= 0 || l == 0.f;           // nothing to average: zeros, whatever the product holds
                 const float2 inv2 = make_float2(1.f / l, 1.f / l);
-                __nv_bfloat16* dst = p.out + (int64_t)(it.q_row[t] + r) * p.o_ts + (int64_t)it.head[t] * p.o_hs;
-                const uint32_t o_addr = tmem + lanes + 256 + t * kPfTile;
-                float2 odd2 = make_float2(0.f, 0.f);               // 0 x (a value that is not finite) is NaN
+                __nv_bfloat16* dst = p.out + (int64_t)(q_row + r) * p.o_ts + (int64_t)head * p.o_hs;
                 float* part = p.part_o + (((size_t)max(it.slot, 0) * 2 + t) * kPfTile + r) * D;
-                uint32_t o[2][16];
-                tm_ld16(o[0], o_addr);
+                uint32_t o_addr = tmem + lanes + 256 + t * kPfTile;
+                float2 odd2 = make_float2(0.f, 0.f);               // 0 x (a value that is not finite) is NaN
+                auto put = [&](const uint32_t (&o)[16]) {          // 16 columns
+                    if (it.slot >= 0) {                            // a piece: as it is, for the join
+                        if (valid) {
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(part), NMT_W8(o, 0) : "memory");
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(part + 8), NMT_W8(o, 8) : "memory");
+                        }
+                        part += 16;
+                        return;
+                    }
+                    uint32_t w[8];
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 f = __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), inv2);
+                        odd2 = __ffma2_rn(f, make_float2(0.f, 0.f), odd2);
+                        w[e] = none ? 0u : pack2(f);
+                    }
+                    if (valid) {
+                        if (p.out32) {
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), NMT_W8(w, 0) : "memory");
+                        } else {
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                    dst += 16;
+                };
+                uint32_t oa[16], ob[16];                           // one is on its way while the other is stored
+                tm_ld16(oa, o_addr);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
                     tm_wait_ld();
-                    if (c + 1 < D / 16) {
-                        tm_ld16(o[(c + 1) & 1], o_addr + 16 * (c + 1));
+                    tm_ld16(ob, o_addr + 16);
+                    put(oa);
+                    tm_wait_ld();
+                    o_addr += 32;
+                    if (c + 32 < D) {
+                        tm_ld16(oa, o_addr);
                     } else {                                       // O and L are in registers: the next item may have them
                         tm_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&bar.o_empty[t]);
                     }
-                    if (it.slot >= 0) {                            // a piece: as it is, for the join
-                        if (r < it.rows[t]) {
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(part + 16 * c), NMT_W8(o[c & 1], 0) : "memory");
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(part + 16 * c + 8), NMT_W8(o[c & 1], 8) : "memory");
-                        }
-                        continue;
-                    }
-                    uint32_t w[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float2 f = __fmul2_rn(make_float2(__uint_as_float(o[c & 1][2 * e]), __uint_as_float(o[c & 1][2 * e + 1])), inv2);
-                        odd2 = __ffma2_rn(f, make_float2(0.f, 0.f), odd2);
-                        w[e] = none ? 0u : pack2(f);
-                    }
-                    if (r < it.rows[t]) {
-                        if (p.out32) {
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 16 * c), NMT_W8(w, 0) : "memory");
-                        } else {
-                            *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4*>(dst + 16 * c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                        }
-                    }
+                    put(ob);
                 }
-                const bool odd = !none && r < it.rows[t] && it.slot < 0 && odd2.x + odd2.y != 0.f;
+                const bool odd = !none && valid && it.slot < 0 && odd2.x + odd2.y != 0.f;
                 for (uint32_t redo = __ballot_sync(0xffffffffu, odd && l < INFINITY); redo; redo &= redo - 1) {
                     const int rr = wq * 32 + __ffs(redo) - 1;
-                    redo_row<D>(p, it.q_row[t] + rr, it.head[t], it.kv_row, p.causal ? min(it.kv_len, it.limit[t] + rr) : it.kv_len);
+                    redo_row<D>(p, q_row + rr, head, it.kv_row, p.causal ? min(it.kv_len, limit + rr) : it.kv_len);
                 }
             }
         }

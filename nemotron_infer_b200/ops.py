@@ -274,13 +274,10 @@ def _on_device(fn):
     return call
 
 
-def _view3(t: torch.Tensor, name: str, rows: int | None, heads: int | None, dim: int, dev) -> tuple[int, int]:
+def _view3(t: torch.Tensor, name: str, rows: int, heads: int, dim: int, dev) -> tuple[int, int]:
     """Checks a bf16 [rows, heads, dim] view (any row and head strides) and returns the two strides."""
-    shape = t.shape
-    if t.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != dim or (rows is not None and shape[0] != rows) or \
-            (heads is not None and shape[1] != heads):
-        raise ValueError(f"{name} must be bf16 [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {dim}], "
-                         f"got {t.dtype} {list(shape)}")
+    if t.dtype is not torch.bfloat16 or t.shape != (rows, heads, dim):
+        raise ValueError(f"{name} must be bf16 [{rows}, {heads}, {dim}], got {t.dtype} {list(t.shape)}")
     rs, hs, es = t.stride()
     if es != 1 and dim > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
@@ -289,58 +286,63 @@ def _view3(t: torch.Tensor, name: str, rows: int | None, heads: int | None, dim:
     return rs, hs
 
 
-def _result3(t: torch.Tensor, name: str, rows: int, heads: int, dim: int, dev) -> tuple[int, int]:
-    """The same for a tensor that is written: no two of its rows may share memory."""
+def _result3(t: torch.Tensor | None, like: torch.Tensor, name: str, rows: int, heads: int, dim: int, dev):
+    """The tensor that takes a result, and its strides: a new one in the shape of `like`, or `t`, of which no two rows may
+    share memory."""
+    if t is None:
+        t = torch.empty_like(like) if like.is_contiguous() else like.new_empty((rows, heads, dim))
+        return t, heads * dim, dim
     rs, hs = _view3(t, name, rows, heads, dim, dev)
-    if t.is_contiguous():
-        return rs, hs
-    spans = sorted(((abs(s), n) for s, n in ((rs, rows), (hs, heads)) if n > 1))
-    need = dim
-    for s, n in spans:
-        if s < need:
-            raise ValueError(f"rows of {name} overlap in memory")
-        need = s * (n - 1) + need
-    return rs, hs
+    if rs != heads * dim or hs != dim:
+        need = dim
+        for s, n in sorted((abs(s), n) for s, n in ((rs, rows), (hs, heads)) if n > 1):
+            if s < need:
+                raise ValueError(f"rows of {name} overlap in memory")
+            need = s * (n - 1) + need
+    return t, rs, hs
 
 
 def _i32(t: torch.Tensor, name: str, dev, shape: tuple[int, ...]) -> int:
     if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
-        raise ValueError(f"{name} must be contiguous int32 {list(shape)} on the caches' device")
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)} on the same device")
     return t.data_ptr()
 
 
+_CACHE_KINDS = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
+
+
 def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
-                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> "_lib.PagedCache":
+                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, dev) -> "_lib.PagedCache":
     """The C descriptor of a paged cache: k_cache / v_cache [num_pages, kv_heads, page_size, head_dim], bf16 or float8_e4m3fn,
-    each page contiguous; page_table int32 [batch, max_pages]; seq_lens int32 [batch]."""
-    dev, shape = k_cache.device, k_cache.shape
-    if k_cache.dtype is torch.bfloat16:
-        kind = 0
-    elif k_cache.dtype is torch.float8_e4m3fn:
-        kind = 1
-    else:
-        raise ValueError("the caches must be bf16 or float8_e4m3fn")
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype or v_cache.device != dev:
-        raise ValueError("k_cache and v_cache must both be [num_pages, kv_heads, page_size, head_dim] of one dtype on one device")
+    each page contiguous; page_table int32 [batch, max_pages]; seq_lens int32 [batch]; all on `dev`."""
+    shape = k_cache.shape
+    kind = _CACHE_KINDS.get(k_cache.dtype)
+    if kind is None or v_cache.dtype is not k_cache.dtype:
+        raise ValueError("the caches must both be bf16 or both float8_e4m3fn")
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError("k_cache and v_cache must both be [num_pages, kv_heads, page_size, head_dim]")
+    if k_cache.device != dev or v_cache.device != dev:
+        raise ValueError("all tensors must live on the same device")
     pages, heads, size, dim = shape
     ks, vs = k_cache.stride(), v_cache.stride()
     for st in (ks, vs):
-        if (dim > 1 and st[3] != 1) or (size > 1 and st[2] != dim) or (heads > 1 and st[1] != size * dim):
+        if st[1:] != (size * dim, dim, 1) and ((dim > 1 and st[3] != 1) or (size > 1 and st[2] != dim) or (heads > 1 and st[1] != size * dim)):
             raise ValueError("every page of a cache must be contiguous [kv_heads, page_size, head_dim]")
     if page_table.dim() != 2:
         raise ValueError("page_table must be int32 [batch, max_pages]")
     batch, max_pages = page_table.shape
+    k_ptr = v_ptr = None
     count = 1
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t is None:
-            continue
-        if t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous() or t.numel() not in (1, heads):
-            raise ValueError(f"{name} must be fp32 with 1 or kv_heads entries on the caches' device")
-        count = t.numel()
-    if k_scale is not None and v_scale is not None and k_scale.numel() != v_scale.numel():
-        raise ValueError("k_scale and v_scale must have the same number of entries")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], vs[0], pages, size, heads, dim, kind,
-                           None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), count,
+    if k_scale is not None or v_scale is not None:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is not None and (t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous() or t.numel() not in (1, heads)):
+                raise ValueError(f"{name} must be fp32 with 1 or kv_heads entries on the caches' device")
+        counts = {t.numel() for t in (k_scale, v_scale) if t is not None}
+        if len(counts) > 1:
+            raise ValueError("k_scale and v_scale must have the same number of entries")
+        count = counts.pop()
+        k_ptr, v_ptr = (None if t is None else t.data_ptr() for t in (k_scale, v_scale))
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], vs[0], pages, size, heads, dim, kind, k_ptr, v_ptr, count,
                            _i32(page_table, "page_table", dev, (batch, max_pages)), _i32(seq_lens, "seq_lens", dev, (batch,)), batch, max_pages)
 
 
@@ -366,13 +368,11 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     rows are not written.  A float8_e4m3fn cache takes value / scale, saturated.  A token whose position, page or rope row
     is out of range writes nothing and sets err_flag (device int32[1])."""
     dev = k.device
-    c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale)
-    if k_cache.device != dev:
-        raise ValueError("all tensors must live on the same device")
+    c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, dev)
     if k.dim() != 3:
         raise ValueError("k must be bf16 [tokens, kv_heads, head_dim]")
-    T = k.shape[0]
-    ks, vs = _view3(k, "k", T, c.kv_heads, c.head_dim, dev), _view3(v, "v", T, c.kv_heads, c.head_dim, dev)
+    T, kv_heads, dim = k.shape[0], k_cache.shape[1], k_cache.shape[3]
+    ks, vs = _view3(k, "k", T, kv_heads, dim, dev), _view3(v, "v", T, kv_heads, dim, dev)
     cu = None if cu_new is None else _i32(cu_new, "cu_new", dev, (c.batch + 1,))
     if cu is None and T != c.batch:
         raise ValueError("without cu_new there is one token per sequence")
@@ -386,10 +386,11 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     if q is not None:
         if rope is None:
             raise ValueError("q is only rotated: it needs rope")
-        qs = _view3(q, "q", T, None, c.head_dim, dev)
+        if q.dim() != 3:
+            raise ValueError("q must be bf16 [tokens, q_heads, head_dim]")
         q_heads = q.shape[1]
-        q_out = q.new_empty(q.shape) if q_out is None else q_out
-        os = _result3(q_out, "q_out", T, q_heads, c.head_dim, dev)
+        qs = _view3(q, "q", T, q_heads, dim, dev)
+        q_out, *os = _result3(q_out, q, "q_out", T, q_heads, dim, dev)
     elif q_out is not None:
         raise ValueError("q_out without q")
     _lib.check(_lib.load().nmt_kv_append_paged_bf16(
@@ -415,23 +416,20 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     scale defaults to 1 / sqrt(head_dim).  A sequence of length 0 gives zeros.  Page ids out of range read as zeros and set
     err_flag (device int32[1]), as does a length past the page table."""
     dev = q.device
-    c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale)
-    if k_cache.device != dev:
-        raise ValueError("all tensors must live on the same device")
+    c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, dev)
     if q.dim() != 3:
         raise ValueError("q must be bf16 [batch, heads, head_dim]")
-    heads = q.shape[1]
-    qs = _view3(q, "q", c.batch, heads, c.head_dim, dev)
-    out = q.new_empty(q.shape) if out is None else out
-    os = _result3(out, "out", c.batch, heads, c.head_dim, dev)
+    batch, heads, kv_heads, dim = page_table.shape[0], q.shape[1], k_cache.shape[1], k_cache.shape[3]
+    qs = _view3(q, "q", batch, heads, dim, dev)
+    out, *os = _result3(out, q, "out", batch, heads, dim, dev)
     lib = _lib.load()
     if workspace is None:
-        workspace = sdpa_decode_paged_workspace(c.batch, heads, c.kv_heads, c.head_dim, dev)
+        workspace = sdpa_decode_paged_workspace(batch, heads, kv_heads, dim, dev)
     elif workspace.device != dev or not workspace.is_contiguous() or \
-            workspace.numel() * workspace.element_size() < lib.nmt_sdpa_decode_paged_workspace_bytes(c.batch, heads, c.kv_heads, c.head_dim):
+            workspace.numel() * workspace.element_size() < lib.nmt_sdpa_decode_paged_workspace_bytes(batch, heads, kv_heads, dim):
         raise ValueError("workspace too small, not contiguous or on another device")
     _lib.check(lib.nmt_sdpa_decode_paged_bf16(c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads,
-                                              c.head_dim ** -0.5 if scale is None else scale,
+                                              dim ** -0.5 if scale is None else scale,
                                               None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), workspace.data_ptr(),
                                               _raw_stream(dev.index)), "sdpa_decode_paged")
     return out
@@ -472,8 +470,7 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: 
             raise ValueError("with cu_seqlens alone, k and v have q's rows")
     elif cu_seqlens_k is not None:
         raise ValueError("cu_seqlens_k without cu_seqlens")
-    out = q.new_empty(q.shape) if out is None else out
-    os = _result3(out, "out", T, heads, dim, dev)
+    out, *os = _result3(out, q, "out", T, heads, dim, dev)
     lib = _lib.load()
     need = lib.nmt_sdpa_prefill_workspace_bytes(batch, T, T_k, heads, kv_heads, dim)
     if need and workspace is None:

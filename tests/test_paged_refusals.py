@@ -95,26 +95,31 @@ def test_descriptor_checks(built_lib):
     bf = torch.bfloat16
     c = torch.zeros(4, 8, 16, 128, dtype=bf)
     t, n = torch.zeros(2, 3, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
-    ok = ops._paged_cache(c, c, t, n, None, None)
+    cpu = c.device
+    ok = ops._paged_cache(c, c, t, n, None, None, cpu)
     assert (ok.num_pages, ok.kv_heads, ok.page_size, ok.head_dim, ok.batch, ok.max_pages, ok.dtype) == (4, 8, 16, 128, 2, 3, 0)
     both = torch.zeros(4, 2, 8, 16, 128, dtype=bf)
-    assert ops._paged_cache(both[:, 0], both[:, 1], t, n, None, None).k_page_stride == 2 * 8 * 16 * 128
+    assert ops._paged_cache(both[:, 0], both[:, 1], t, n, None, None, cpu).k_page_stride == 2 * 8 * 16 * 128
     one = torch.ones(1)
     for args in ((c.float(), c.float(), t, n, None, None), (c, c[:3], t, n, None, None), (c[0], c[0], t, n, None, None),
                  (c.transpose(1, 2), c.transpose(1, 2), t, n, None, None), (c, c, t.long(), n, None, None), (c, c, t[0], n, None, None),
                  (c, c, t, n[:1], None, None), (c, c, t, n.float(), None, None), (c, c, t.t(), n, None, None), (c, c, t, n, torch.ones(3), None),
                  (c, c, t, n, one.double(), None), (c, c, t, n, one, torch.ones(8)), (c, c.to(torch.float8_e4m3fn), t, n, None, None)):
         with pytest.raises(ValueError):
-            ops._paged_cache(*args)
+            ops._paged_cache(*args, cpu)
+    with pytest.raises(ValueError, match="same device"):
+        ops._paged_cache(c, c, t, n, None, None, torch.device("cuda", 0))
     x = torch.zeros(5, 8, 128, dtype=bf)
     assert ops._view3(x, "x", 5, 8, 128, x.device) == (1024, 128)
     assert ops._view3(torch.zeros(8, 5, 128, dtype=bf).transpose(0, 1), "x", 5, 8, 128, x.device) == (128, 640)
     for bad in (x.float(), x[0], x[:4], x[:, :7], x[..., :64], torch.zeros(5, 8, 256, dtype=bf)[..., ::2], x[..., None]):
         with pytest.raises(ValueError):
             ops._view3(bad, "x", 5, 8, 128, x.device)
+    new, *strides = ops._result3(None, x.transpose(0, 1).contiguous().transpose(0, 1), "out", 5, 8, 128, x.device)
+    assert new.is_contiguous() and strides == [1024, 128]
     for overlapping in (x[:1].expand(5, 8, 128), x[:, :1].expand(5, 8, 128), torch.zeros(4096, dtype=bf).as_strided((5, 8, 128), (8, 128, 1))):
         with pytest.raises(ValueError, match="overlap"):
-            ops._result3(overlapping, "out", 5, 8, 128, x.device)
+            ops._result3(overlapping, x, "out", 5, 8, 128, x.device)
 
 
 def test_rope_table_is_exact_at_far_positions():
