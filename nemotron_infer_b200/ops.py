@@ -321,16 +321,22 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
         raise ValueError("the caches must both be bf16 or both float8_e4m3fn")
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must both be [num_pages, kv_heads, page_size, head_dim]")
-    if k_cache.device != dev or v_cache.device != dev:
-        raise ValueError("all tensors must live on the same device")
     pages, heads, size, dim = shape
     ks, vs = k_cache.stride(), v_cache.stride()
-    for st in (ks, vs):
-        if st[1:] != (size * dim, dim, 1) and ((dim > 1 and st[3] != 1) or (size > 1 and st[2] != dim) or (heads > 1 and st[1] != size * dim)):
-            raise ValueError("every page of a cache must be contiguous [kv_heads, page_size, head_dim]")
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be int32 [batch, max_pages]")
-    batch, max_pages = page_table.shape
+    inner = (size * dim, dim, 1)
+    if ks[1:] != inner or vs[1:] != inner:
+        for st in (ks, vs):
+            if (dim > 1 and st[3] != 1) or (size > 1 and st[2] != dim) or (heads > 1 and st[1] != size * dim):
+                raise ValueError("every page of a cache must be contiguous [kv_heads, page_size, head_dim]")
+    try:
+        batch, max_pages = page_table.shape
+    except ValueError:
+        raise ValueError("page_table must be int32 [batch, max_pages]") from None
+    if page_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32 or seq_lens.shape != (batch,) or \
+            not (page_table.is_contiguous() and seq_lens.is_contiguous()):
+        raise ValueError(f"page_table must be contiguous int32 [batch, max_pages] and seq_lens contiguous int32 [{batch}]")
+    if k_cache.device != dev or v_cache.device != dev or page_table.device != dev or seq_lens.device != dev:
+        raise ValueError("all tensors must live on the same device")
     k_ptr = v_ptr = None
     count = 1
     if k_scale is not None or v_scale is not None:
@@ -343,7 +349,12 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
         count = counts.pop()
         k_ptr, v_ptr = (None if t is None else t.data_ptr() for t in (k_scale, v_scale))
     return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], vs[0], pages, size, heads, dim, kind, k_ptr, v_ptr, count,
-                           _i32(page_table, "page_table", dev, (batch, max_pages)), _i32(seq_lens, "seq_lens", dev, (batch,)), batch, max_pages)
+                           page_table.data_ptr(), seq_lens.data_ptr(), batch, max_pages)
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(name: str, *sizes: int) -> int:
+    return int(getattr(_lib.load(), name)(*sizes))
 
 
 def rope_table(positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -402,8 +413,8 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
 def sdpa_decode_paged_workspace(batch: int, heads: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
     """Workspace of sdpa_decode_paged for these sizes; calls that may overlap on the GPU need one each."""
-    need = _lib.load().nmt_sdpa_decode_paged_workspace_bytes(batch, heads, kv_heads, head_dim)
-    return torch.empty(max(int(need), 16), dtype=torch.uint8, device=device)
+    return torch.empty(max(_workspace_bytes("nmt_sdpa_decode_paged_workspace_bytes", batch, heads, kv_heads, head_dim), 16), dtype=torch.uint8,
+                       device=device)
 
 
 @_on_device
@@ -422,13 +433,12 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     batch, heads, kv_heads, dim = page_table.shape[0], q.shape[1], k_cache.shape[1], k_cache.shape[3]
     qs = _view3(q, "q", batch, heads, dim, dev)
     out, *os = _result3(out, q, "out", batch, heads, dim, dev)
-    lib = _lib.load()
     if workspace is None:
         workspace = sdpa_decode_paged_workspace(batch, heads, kv_heads, dim, dev)
     elif workspace.device != dev or not workspace.is_contiguous() or \
-            workspace.numel() * workspace.element_size() < lib.nmt_sdpa_decode_paged_workspace_bytes(batch, heads, kv_heads, dim):
+            workspace.numel() * workspace.element_size() < _workspace_bytes("nmt_sdpa_decode_paged_workspace_bytes", batch, heads, kv_heads, dim):
         raise ValueError("workspace too small, not contiguous or on another device")
-    _lib.check(lib.nmt_sdpa_decode_paged_bf16(c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads,
+    _lib.check(_lib.load().nmt_sdpa_decode_paged_bf16(c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads,
                                               dim ** -0.5 if scale is None else scale,
                                               None if err_flag is None else _i32(err_flag, "err_flag", dev, (1,)), workspace.data_ptr(),
                                               _raw_stream(dev.index)), "sdpa_decode_paged")
