@@ -49,7 +49,7 @@ struct DecodeArgs {
     const int32_t *seq_lens, *page_table;
     const float *k_scale, *v_scale;
     int32_t* err_flag;
-    int4* desc;                                                    // [kDecCtas][2]: what CTA c's piece starts with
+    int4* desc;                                                    // [kDecCtas][2]: where CTA c starts, and what the join needs to know of it
     float2* ml;                                                    // [kDecCtas][2][heads of a unit]: maximum (log 2 units), sum
     float* o;                                                      // [kDecCtas][2][heads of a unit][D]
     float scale_log2;
@@ -194,13 +194,10 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
         auto share = [&](int64_t places, const Cursor& k) {
             return static_cast<int>(min((int64_t)(k.tiles - k.tile), k.tile == 0 ? places - kUnitCost : places));
         };
-        if (threadIdx.x == 0) {
-            p.desc[2 * blockIdx.x] = make_int4(c.b, c.unit, c.tile, c.tiles);
-            p.desc[2 * blockIdx.x + 1] = make_int4(ctas, 0, static_cast<int>(total & 0xffffffff), static_cast<int>(total >> 32));
-        }
         if (warp == kDecWarps) {
             // ---------------- producer ----------------
             const int page_rows = 1 << p.page_shift, box_rows = min(page_rows, TK);
+            const int4 cut = make_int4(c.b, c.unit, c.tile, c.tiles);
             int n = 0;
             bool ok = true;
             for (int take; ok && (take = share(left, c)) > 0;) {
@@ -233,6 +230,18 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
                     ++c.tile;
                 }
                 if (c.tile == c.tiles) c.next_unit(p);
+            }
+            if (lane == 0) {
+                // For the join: if this is the first cut inside a unit, how many pieces the unit has, this CTA's and the one before
+                // it included, and whether the piece before is that CTA's first.
+                int pieces = 0, slot = 0;
+                if (cut.z > 0) {
+                    const int64_t before_this = begin - (int64_t)(blockIdx.x - 1) * total / ctas, unit_end = begin + (cut.w - cut.z);
+                    if (cut.z <= before_this) pieces = static_cast<int>((unit_end * ctas + total - 1) / total) - static_cast<int>(blockIdx.x) + 1;
+                    slot = cut.z + kUnitCost >= before_this ? 0 : 1;
+                }
+                p.desc[2 * blockIdx.x] = cut;
+                p.desc[2 * blockIdx.x + 1] = make_int4(ctas, pieces, slot, 0);
             }
             for (int s = max(0, n - kDecStages); s < n; ++s) mbar_wait(&s_full[s % kDecStages], static_cast<uint32_t>(s / kDecStages) & 1u);
         } else {
@@ -524,7 +533,7 @@ sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
 }
 
 // Joins the pieces of the units that were cut.  CTA (c - 1, r) belongs to the cut between ranges c - 1 and c; it works if
-// that is the FIRST cut inside the unit there, and joins query head r of it: pieces c - 1 (its last), c, c + 1, ...
+// that is the FIRST cut inside the unit there, and joins query head r of it: pieces c - 1, c, c + 1, ...
 // Nothing here is long, so the chain of dependent loads counts: what cut this is -> maxima, sums and outputs, all at once.
 // A warp takes every eighth piece, a lane D / 32 columns of it; every warp works out the weights for itself.
 constexpr int kJoinWarps = 8;
@@ -536,18 +545,12 @@ sdpa_decode_paged_join_kernel(const DecodeArgs p, int hpu) {
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x + 1, r = blockIdx.y;
-    const int4 line = p.desc[1], cut = p.desc[2 * c];
-    const int ctas = line.x;
-    const int64_t total = ((int64_t)line.w << 32) | (uint32_t)line.z;
-    if (c < ctas) {
-        const int64_t start = (int64_t)c * total / ctas, start_prev = (int64_t)(c - 1) * total / ctas;
-        const int f = cut.z, tiles = cut.w, b = cut.x, unit = cut.y;
+    const int ctas = p.desc[1].x;
+    const int4 cut = p.desc[2 * c], join = p.desc[2 * c + 1];
+    if (c < ctas && join.y > 0) {
+        const int b = cut.x, unit = cut.y, n = join.y, slot0 = join.z;
         const int head = unit / p.chunks, q0 = (unit % p.chunks) * hpu, heads = min(hpu, p.group - q0);
-        if (f > 0 && f <= start - start_prev && r < heads) {
-            const int64_t unit_end = start + (tiles - f);
-            const int last = static_cast<int>((unit_end * ctas + total - 1) / total) - 1;       // range that holds its last tile
-            const int n = last - (c - 1) + 1;
-            const int slot0 = f + kUnitCost >= start - start_prev ? 0 : 1;         // was the unit the first of range c - 1
+        if (r < heads) {
             auto piece = [&](int i) { return ((size_t)(c - 1 + i) * 2 + (i == 0 ? slot0 : 0)) * hpu + r; };
             using Cols = typename std::conditional<D == 128, float4, float2>::type;
             Cols ahead[AHEAD];
