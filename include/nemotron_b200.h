@@ -242,7 +242,7 @@ int nmt_sdpa_decode_bf16(const void* Q, void* K_cache, void* V_cache, void* O, c
  * the reference, whose cache is one contiguous buffer for one sequence (tensor layout of ops/attention/sdpa_decode.cuh).
  *   page_size  a power of two, 8 .. 1024;  head_dim 64 or 128;  k, v 16-byte aligned, page strides multiples of 16 bytes
  *   dtype      NMT_CACHE_BF16, or NMT_CACHE_E4M3: an element stands for its value times the scale
- *   k_scale, v_scale   device fp32, scale_count of them: 1 (per tensor) or kv_heads; NULL = 1.0
+ *   k_scale, v_scale   device fp32, scale_count of them: 1 (per tensor) or kv_heads; NULL = 1.0.  e4m3 caches only
  *   page_table device int32 [batch][max_pages];  seq_lens device int32 [batch]: tokens of each sequence, the ones that
  *              the call appends included.  Both are read by the kernels, not by the host: a captured graph may be replayed
  *              with other contents.

@@ -16,6 +16,7 @@ inline int check_paged_cache(const nmt_paged_cache* c) {
     if (c->dtype != NMT_CACHE_BF16 && c->dtype != NMT_CACHE_E4M3) return NMT_ERR_UNSUPPORTED;
     if ((c->head_dim != 64 && c->head_dim != 128) || !pow2(c->page_size) || c->page_size < 8 || c->page_size > 1024) return NMT_ERR_UNSUPPORTED;
     if (c->kv_heads > 65535 || c->batch > 0x3fffffff || c->num_pages > 0x7fffffff || c->max_pages > 0x7fffffff / c->page_size) return NMT_ERR_UNSUPPORTED;
+    if ((c->k_scale || c->v_scale) && c->dtype == NMT_CACHE_BF16) return NMT_ERR_UNSUPPORTED;
     if ((c->k_scale || c->v_scale) && c->scale_count != 1 && c->scale_count != c->kv_heads) return NMT_ERR_SHAPE;
     const int64_t page = c->kv_heads * c->page_size * c->head_dim, per16 = c->dtype == NMT_CACHE_BF16 ? 8 : 16;
     if (c->num_pages > 1 && (c->k_page_stride < page || c->v_page_stride < page)) return NMT_ERR_SHAPE;

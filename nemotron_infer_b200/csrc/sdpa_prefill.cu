@@ -133,13 +133,13 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x on the FMA pipe, two at a time, for -inf < x < 128 (results below 2^-125 come out as 2^-125).  x = n + f with n the
-// nearest integer (adding 1.5 * 2^23 leaves it in the low bits of the sum), f in [-1/2, 1/2], and 2^f by a polynomial of
+// 2^x on the FMA pipe, two at a time, for -inf < x < 128.  x is kept at or above -127, where the result is an exact zero (and
+// between there and -126 anything below 2^-126).  x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits of the sum), f in [-1/2, 1/2], and 2^f by a polynomial of
 // degree 4 with constant term 1, fitted for the least relative error (minimax, by linear programming): 2.9e-6 = 2^-18.4,
 // against the 2^-8 of the rounding to bf16 that follows.  n goes into the exponent by an integer addition.
 __device__ __forceinline__ float2 ex2_fma(const float2& x) {
     const float2 magic = make_float2(12582912.f, 12582912.f);
-    const float2 xc = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+    const float2 xc = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
     const float2 t = __fadd2_rn(xc, magic);
     const float2 f = __fadd2_rn(xc, __ffma2_rn(t, make_float2(-1.f, -1.f), magic));
     float2 y = __ffma2_rn(f, make_float2(0.009582576341927052f, 0.009582576341927052f), make_float2(0.05590682849287987f, 0.05590682849287987f));

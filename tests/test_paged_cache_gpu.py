@@ -133,6 +133,22 @@ def test_append_specials(ops):
     assert math.isnan(got[0].item()) and got[1:5].tolist() == [448.0, -448.0, 448.0, -448.0] and not bool(got[5:].any())
 
 
+@pytest.mark.parametrize("scale", [1.0, 0.75, 0.1, 3e-3, 2.0 ** -14, 2.0 ** -15, 1e-5, 1e-32, 7.0, 1e4, 3e31, -0.5])
+def test_append_quotients_are_a_divisions(ops, scale):
+    """Every bf16 value over a scale: the same e4m3 value as dividing in fp32 and rounding, ties included."""
+    bits = torch.arange(65536, dtype=torch.int32, device="cuda").to(torch.int16)
+    x = bits.view(BF).view(1024, 1, 64)
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8)
+    kc, vc = (torch.zeros(8, 1, 128, 64, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    s = torch.full((1,), scale, device="cuda")
+    ops.kv_append_paged(x, x, kc, vc, table, torch.full((1,), 1024, dtype=torch.int32, device="cuda"),
+                        torch.tensor([0, 1024], dtype=torch.int32, device="cuda"), k_scale=s, v_scale=s)
+    want = (x.float() / s).clamp(-448, 448).to(E4M3).float()
+    for c in (kc, vc):
+        got = c.view(1024, 1, 64).float()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
 def test_append_out_of_range_writes_nothing_and_reports(ops):
     g = gen(6)
     k = randn(g, 4, 2, 64).to(BF)

@@ -21,7 +21,7 @@ BAD_CACHES = [
     (dict(page_size=12), UNSUPPORTED), (dict(page_size=4), UNSUPPORTED), (dict(page_size=2048), UNSUPPORTED), (dict(head_dim=96), UNSUPPORTED),
     (dict(dtype=2), UNSUPPORTED), (dict(num_pages=0), SHAPE), (dict(max_pages=0), SHAPE), (dict(kv_heads=0), SHAPE), (dict(batch=-1), SHAPE),
     (dict(k_page_stride=8 * 16 * 128 - 8), SHAPE), (dict(v_page_stride=8 * 16 * 128 + 4), ALIGN), (dict(k=BUF + 8), ALIGN), (dict(v=BUF + 2), ALIGN),
-    (dict(page_table=BUF + 2), ALIGN), (dict(k_scale=BUF, scale_count=3), SHAPE), (dict(k_scale=BUF + 1), ALIGN), (dict(max_pages=1 << 28), UNSUPPORTED),
+    (dict(page_table=BUF + 2), ALIGN), (dict(k_scale=BUF, scale_count=3, dtype=1), SHAPE), (dict(k_scale=BUF + 1, dtype=1), ALIGN), (dict(k_scale=BUF), UNSUPPORTED), (dict(v_scale=BUF), UNSUPPORTED), (dict(max_pages=1 << 28), UNSUPPORTED),
     (dict(k=None), NULL), (dict(v=None), NULL), (dict(page_table=None), NULL), (dict(seq_lens=None), NULL),
 ]
 

@@ -124,6 +124,18 @@ def test_growing_maximum(ops):
     compare(ops.sdpa_prefill(q, k, v, causal=False), q, k, v, [n], [n], False, dim ** -0.5)
 
 
+def test_negligible_weights_are_zeros(ops):
+    """Keys more than 2^127 below the row's largest weight count for nothing, however large their values."""
+    n, dim = 512, 64
+    q = torch.ones(n, 1, dim, dtype=BF, device="cuda")
+    k = torch.zeros(n, 1, dim, dtype=BF, device="cuda")
+    k[1::2] = -4.0                                                  # scores 0 and -4 * 64 * 8 in turn
+    v = torch.ones(n, 1, dim, dtype=BF, device="cuda")
+    v[1::2] = 3e38
+    out = ops.sdpa_prefill(q, k, v, causal=False, scale=8.0)
+    assert bool((out == 1).all())
+
+
 def test_views_padding_and_out(ops):
     """q, k, v as views of one projection's output, out transposed, padding rows untouched, an explicit scale."""
     g = gen(7)
