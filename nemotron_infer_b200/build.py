@@ -86,7 +86,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_pybind(force: bool = False) -> str:
-    """Compiles nemotron_infer_b200/pybind/binding.cpp into an importable module next to it, linked to the library."""
+    """Compiles nemotron_infer_b200/pybind/binding.cpp into an importable module next to it, linked to the library, and the
+    compiled tensor-level calls (build_torch_calls)."""
     import sysconfig
     import pybind11
     build()
@@ -99,6 +100,30 @@ def build_pybind(force: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"pybind module failed to build:\n{r.stdout}\n{r.stderr}")
+    build_torch_calls(force)
+    return out
+
+
+def build_torch_calls(force: bool = False) -> str:
+    """Compiles nemotron_infer_b200/torch_ext/paged_calls.cpp into an importable module of the package, linked to the library
+    and to the installed torch."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    build()
+    src = os.path.join(PKG_DIR, "torch_ext", "paged_calls.cpp")
+    out = os.path.join(PKG_DIR, "_paged_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+    if force or _stale(out, [src, os.path.join(INCLUDE, "nemotron_b200.h"), torch.__file__]):
+        lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+        for d in [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], cuda, INCLUDE]:
+            cmd += ["-isystem" if d != INCLUDE else "-I", d]
+        cmd += [src, "-o", out, "-L", PKG_DIR, "-lnemotron_b200", "-Wl,-rpath,$ORIGIN", "-L", lib, f"-Wl,-rpath,{lib}",
+                "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"paged_calls failed to build:\n{r.stdout}\n{r.stderr}")
     return out
 
 
@@ -106,7 +131,7 @@ def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--verbose", action="store_true", help="print ptxas register/spill reports")
-    ap.add_argument("--pybind", action="store_true", help="also build the pybind11 module nemotron_infer_b200.pybind.binding")
+    ap.add_argument("--pybind", action="store_true", help="also build the compiled modules: nemotron_infer_b200.pybind.binding and the tensor-level calls")
     a = ap.parse_args()
     print(build(force=a.force, verbose=a.verbose))
     if a.pybind:

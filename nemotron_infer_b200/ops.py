@@ -259,6 +259,16 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# The compiled calls (torch_ext/paged_calls.cpp) take the usual arguments of the three operators below as they are, with the same
+# checks; what they hand back (Ellipsis) is gone through here, step by step.
+try:
+    from . import _paged_calls
+    if torch.__version__.split("+")[0] != _paged_calls.torch_version:
+        _paged_calls = None
+except ImportError:
+    _paged_calls = None
+
+
 def _on_device(fn):
     """The operators over strided views and caches may be called with tensors of a device that is not the current one: they
     run on that device, on its current stream."""
@@ -365,7 +375,6 @@ def rope_table(positions: int, rot_dim: int, base: float = 10000.0, device="cuda
     return torch.cat([a.cos(), a.sin()], dim=1).to(dtype=torch.float32).to(device)
 
 
-@_on_device
 def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     seq_lens: torch.Tensor, cu_new: torch.Tensor | None = None, q: torch.Tensor | None = None,
                     rope: torch.Tensor | None = None, interleaved: bool = False, k_scale: torch.Tensor | None = None,
@@ -378,6 +387,15 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     [tokens, q_heads, head_dim] when given: the result is q_out (q itself, for in place) or a new tensor, whose padding
     rows are not written.  A float8_e4m3fn cache takes value / scale, saturated.  A token whose position, page or rope row
     is out of range writes nothing and sets err_flag (device int32[1])."""
+    if _paged_calls is not None:
+        r = _paged_calls.kv_append_paged(k, v, k_cache, v_cache, page_table, seq_lens, cu_new, q, rope, interleaved, k_scale, v_scale, q_out, err_flag)
+        if r is not ...:
+            return r if type(r) is not int else _lib.check(r, "kv_append_paged")
+    return _kv_append_paged(k, v, k_cache, v_cache, page_table, seq_lens, cu_new, q, rope, interleaved, k_scale, v_scale, q_out, err_flag)
+
+
+@_on_device
+def _kv_append_paged(k, v, k_cache, v_cache, page_table, seq_lens, cu_new, q, rope, interleaved, k_scale, v_scale, q_out, err_flag):
     dev = k.device
     c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, dev)
     if k.dim() != 3:
@@ -417,7 +435,6 @@ def sdpa_decode_paged_workspace(batch: int, heads: int, kv_heads: int, head_dim:
                        device=device)
 
 
-@_on_device
 def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                       scale: float | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                       out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
@@ -426,6 +443,15 @@ def sdpa_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     positions of its pages (the caches and tables kv_append_paged writes; append first, then the token sees itself).
     scale defaults to 1 / sqrt(head_dim).  A sequence of length 0 gives zeros.  Page ids out of range read as zeros and set
     err_flag (device int32[1]), as does a length past the page table."""
+    if _paged_calls is not None:
+        r = _paged_calls.sdpa_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale, v_scale, out, workspace, err_flag)
+        if r is not ...:
+            return r if type(r) is not int else _lib.check(r, "sdpa_decode_paged")
+    return _sdpa_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale, v_scale, out, workspace, err_flag)
+
+
+@_on_device
+def _sdpa_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale, v_scale, out, workspace, err_flag):
     dev = q.device
     c = _paged_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, dev)
     if q.dim() != 3:
@@ -451,7 +477,6 @@ def sdpa_prefill_workspace(batch: int, tokens: int, kv_tokens: int, heads: int, 
                        device=device)
 
 
-@_on_device
 def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
                  cu_seqlens_k: torch.Tensor | None = None, causal: bool = True, scale: float | None = None,
                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -461,6 +486,15 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: 
     queries and m keys sees keys j <= i + (m - n): a sequence whose first part is cached passes more keys than queries.  A
     query that sees nothing gives zeros.  Rows behind the last sequence are not written.  scale defaults to
     1 / sqrt(head_dim).  workspace: sdpa_prefill_workspace(...), which is empty for most sizes; allocated here if not given."""
+    if _paged_calls is not None:
+        r = _paged_calls.sdpa_prefill(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, out, workspace)
+        if r is not ...:
+            return r if type(r) is not int else _lib.check(r, "sdpa_prefill")
+    return _sdpa_prefill(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, out, workspace)
+
+
+@_on_device
+def _sdpa_prefill(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, out, workspace):
     dev = q.device
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q, k and v must be bf16 [tokens, heads, head_dim]")

@@ -1,0 +1,125 @@
+"""The two ways into the paged cache operators and prompt attention - the compiled calls and the checks step by step - take and refuse the
+same arguments and give the same bits; two calls at once on two streams do not disturb each other."""
+import math
+
+import pytest
+import torch
+
+from paged_common import BF, gen, pages_for
+from paged_common import randn as randn32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(built_lib):
+    from nemotron_infer_b200 import ops as _ops
+    assert torch.cuda.is_available()
+    built_lib.nmt_set_device(torch.cuda.current_device())
+    yield _ops
+    torch.cuda.synchronize()
+    assert built_lib.nmt_device_wait_timeouts() == 0
+
+
+def randn(g, *shape):
+    return randn32(g, *shape).to(BF)
+
+
+def step(g, lens, heads=8, kv_heads=2, dim=128, page=16, dtype=BF):
+    table, num = pages_for(lens, page, g)
+    kc, vc = (randn(g, num, kv_heads, page, dim).to(dtype) for _ in range(2))
+    B = len(lens)
+    return dict(q=randn(g, B, heads, dim), k=randn(g, B, kv_heads, dim), v=randn(g, B, kv_heads, dim), kc=kc, vc=vc, table=table,
+                lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+
+
+def calls(ops, s, **over):
+    """The three operators on one step's tensors: what each gives, or the error it raises."""
+    s = {**s, **over}
+    kc, vc = s["kc"].clone(memory_format=torch.preserve_format), s["vc"].clone(memory_format=torch.preserve_format)
+    got = []
+    for call in (lambda: (ops.kv_append_paged(s["k"], s["v"], kc, vc, s["table"], s["lens"], s.get("cu"), s["q"], s.get("rope"), s.get("interleaved", False),
+                                              s.get("ks"), s.get("vs"), s.get("q_out"), s.get("err")), kc, vc),
+                 lambda: ops.sdpa_decode_paged(s["q"], kc, vc, s["table"], s["lens"], s.get("scale"), s.get("ks"), s.get("vs"), s.get("out"),
+                                               s.get("ws"), s.get("err")),
+                 lambda: ops.sdpa_prefill(s["q"], s["k"], s["v"], s.get("cu"), s.get("cu_k"), s.get("causal", True), s.get("scale"), s.get("out"),
+                                          s.get("ws"))):
+        try:
+            r = call()
+            got += [t.clone() for t in (r if isinstance(r, tuple) else (r,)) if t is not None]
+        except (ValueError, RuntimeError) as e:
+            got.append((type(e).__name__, str(e)))
+    return got
+
+
+def same(a, b, what):
+    assert len(a) == len(b), what
+    for x, y in zip(a, b):
+        if isinstance(x, torch.Tensor):
+            assert isinstance(y, torch.Tensor) and x.dtype == y.dtype and x.shape == y.shape, what
+            bits = {1: torch.uint8, 2: torch.int16}[x.element_size()]
+            assert torch.equal(x.contiguous().view(bits), y.contiguous().view(bits)), what
+        else:
+            assert x == y, (what, x, y)
+
+
+def test_both_ways_agree(ops, monkeypatch):
+    if ops._paged_calls is None:
+        pytest.skip("the compiled calls are not built")
+    g = gen(5)
+    s = step(g, [1, 40, 3, 77])
+    s["rope"] = ops.rope_table(100, 128)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    f32 = lambda *v: torch.tensor(v, dtype=torch.float32, device="cuda")
+    e4m3 = {"kc": s["kc"].to(torch.float8_e4m3fn), "vc": s["vc"].to(torch.float8_e4m3fn)}
+    wide = torch.empty(4, 12, 160, dtype=BF, device="cuda")
+    overs = [
+        {}, {"interleaved": True}, {"rope": None}, {"scale": 0.3}, {"scale": 1}, {"scale": math.nan}, {"causal": False},
+        {"cu": i32(0, 1, 2, 3, 4)}, {"cu": i32(0, 1, 1, 1, 4)}, {"cu": i32(0, 4)}, {"cu": i32()}, {"cu": i32(0, 1, 2, 3, 4).long()},
+        {"cu": i32(0, 1, 2, 3, 4), "cu_k": i32(0, 0, 2, 3, 4)}, {"cu_k": i32(0, 1, 2, 3, 4)},
+        e4m3, {**e4m3, "ks": f32(0.5), "vs": f32(2.0)}, {**e4m3, "ks": f32(0.5, 0.25)}, {**e4m3, "ks": f32(0.5, 0.25), "vs": f32(2.0)},
+        {**e4m3, "ks": f32(1.0, 1.0, 1.0)}, {"ks": f32(0.5)}, {"kc": e4m3["kc"]},
+        {"q": wide[:, 1:9, 8:136]}, {"q": wide[:, 1:9, 3:131]}, {"q": s["q"].float()}, {"q": s["q"][:3]}, {"q": s["q"][:, :3]}, {"q": s["q"][0]},
+        {"k": s["k"].transpose(1, 2).contiguous().transpose(1, 2)}, {"k": s["k"][..., :64]}, {"v": s["v"].cpu()}, {"k": s["k"][:, :1]},
+        {"out": torch.empty(4, 8, 128, dtype=BF, device="cuda")}, {"out": wide[:, 4:, :128]}, {"out": wide[:1, :8, :128].expand(4, 8, 128)},
+        {"q_out": torch.empty(4, 8, 128, dtype=BF, device="cuda")}, {"out": torch.empty(4, 8, 128, device="cuda")},
+        {"ws": torch.empty(16, dtype=torch.uint8, device="cuda")}, {"ws": torch.empty(64 << 20, dtype=torch.uint8, device="cuda")},
+        {"err": i32(0)}, {"err": i32(0, 0)}, {"table": s["table"].long()}, {"table": s["table"][:3]}, {"lens": s["lens"][:3]},
+        {"lens": s["lens"].cpu()}, {"rope": s["rope"].double()}, {"rope": s["rope"][:, :24].contiguous()}, {"rope": s["rope"][:, ::2]},
+        {"kc": s["kc"][:, :, :12], "vc": s["vc"][:, :, :12]}, {"kc": s["kc"].transpose(1, 2), "vc": s["vc"].transpose(1, 2)},
+        {"k": torch.nn.Parameter(s["k"], requires_grad=False)},
+    ]
+    good = 0
+    for n, over in enumerate(overs):
+        compiled = calls(ops, s, **over)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_paged_calls", None)
+            stepwise = calls(ops, s, **over)
+        # err_flag and out are shared by both runs on purpose: the same results are written again
+        same(compiled, stepwise, (n, list(over)))
+        good += all(isinstance(x, torch.Tensor) for x in compiled)
+    assert good >= 10
+
+
+def test_two_streams_at_once(ops):
+    """Steps of two batches, each on its own stream with its own workspace, over and over: the results of running alone."""
+    g = gen(6)
+    sets = [step(g, [3000, 17, 900], dim=128), step(g, [5, 2100, 64, 700, 1, 0], dim=64, heads=16, kv_heads=4)]
+    qs = [randn(g, 700, 8, 128), randn(g, 700, 16, 64)]
+    ks = [randn(g, 6000, 2, 128), randn(g, 6000, 4, 64)]
+    alone = [(ops.sdpa_decode_paged(s["q"], s["kc"], s["vc"], s["table"], s["lens"]),
+              ops.sdpa_prefill(q, k, k, torch.tensor([0, 700], dtype=torch.int32, device="cuda"), torch.tensor([0, 6000], dtype=torch.int32, device="cuda")))
+             for s, q, k in zip(sets, qs, ks)]
+    cu = torch.tensor([0, 700], dtype=torch.int32, device="cuda")
+    cu_k = torch.tensor([0, 6000], dtype=torch.int32, device="cuda")
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (s, q, k, st) in enumerate(zip(sets, qs, ks, streams)):
+            with torch.cuda.stream(st):
+                got[i].append((ops.sdpa_decode_paged(s["q"], s["kc"], s["vc"], s["table"], s["lens"]), ops.sdpa_prefill(q, k, k, cu, cu_k)))
+    torch.cuda.synchronize()
+    for i, want in enumerate(alone):
+        for d, p in got[i]:
+            assert torch.equal(d, want[0]) and torch.equal(p, want[1])
