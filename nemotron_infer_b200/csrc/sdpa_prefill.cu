@@ -11,7 +11,8 @@
 //   warps 0-3, 4-7   softmax of query tile 0 / 1: a thread owns a row.  Reads S from tensor memory, writes P (bf16) over it
 //   warps 8-11       epilogue: O / L -> bf16 -> global memory, while the other warps are at the next item already
 //   warp 12          issues the MMAs (one lane)
-//   warp 13          producer: finds the next item, publishes it, and copies its Q, K, V into shared memory (tensor maps)
+//   warp 13          producer: copies Q, K, V of the items into shared memory (tensor maps)
+//   warp 14          scheduler: finds the next item and publishes it
 // S_t = Q_t K^T: tcgen05.mma 128 x 128 x 16 from shared memory (both operands rows of 128 bytes, 128-byte swizzle) into
 // tensor memory.  O_t += P_t V: A comes from tensor memory, where P_t lies over S_t's first 64 columns, B is V as it lies
 // in memory (keys x head_dim, so MN-major).  Columns 0-127 S_0 / P_0, 128-255 S_1 / P_1, 256-383 O_0, 384-511 O_1: all 512.
@@ -37,6 +38,10 @@ constexpr int kPfSlack = 4;                                        // an item th
 constexpr int kPfPieces = 2 * kSmCount;                            // pieces there can be (see pieces())
 constexpr int kPfSplitItems = 4 * kSmCount;                        // with more items than this nothing is cut
 
+// An item of more K / V tiles than this is followed by asking for the next one when its last tiles go out, not earlier - whoever
+// is free shall have it; with fewer the next one is asked for at once, since finding it takes as long as the item.
+constexpr int kPfEager = 2;
+
 template <int D>
 struct PfShape {
     static constexpr int kTileBytes = kPfTile * D * 2;             // Q tile, K tile or V tile
@@ -45,25 +50,49 @@ struct PfShape {
     static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
 };
 
+// x / d for 0 <= x < 2^31 by a multiplication: d = 1 .. 2^16 is the same for a whole launch, and the order of the items is
+// worked out while everybody waits for the first one (with the machine's division one prompt of 2048 tokens took 61 us, not 50).
+struct PfDivide {
+    uint32_t by = 0, log = 0;                      // ceil(2^(31 + log) / d) with log = ceil(log2 d): too large by less than 2^-31 relative
+    static PfDivide of(int64_t d) {
+        PfDivide r;
+        while (((int64_t)1 << r.log) < d) ++r.log;
+        r.by = static_cast<uint32_t>((((uint64_t)1 << (31 + r.log)) + d - 1) / d);
+        return r;
+    }
+    __device__ __forceinline__ int operator()(int x) const { return static_cast<int>(__umulhi(static_cast<uint32_t>(x) << 1, by) >> log); }
+};
+
+struct PfItem {
+    int kv_row;                                    // first key of the sequence in k and v
+    int kv_len, kv_head;
+    int packed;                                    // 0: tile row r is query row r of one head; 1: query row r / group, head r % group
+    // per query tile: first row in q and out, valid tile rows (1 .. 128), keys that query row 0 sees before clamping (row i sees
+    // limit + i when causal), (first) head, K / V tiles.  n[0] < 0: no more items; n[1] == 0: one query tile only.  n[0] <= n[1]
+    // otherwise.
+    int q_row[2], rows[2], limit[2], head[2], n[2];
+    int first;                                     // first K / V tile: 0 unless this is a piece of a cut item
+    int slot;                                      // where a piece leaves its result; < 0: a whole item, written to out
+};
+
+// What the join needs: of every number below kPfPieces, whether it is the first piece of an item, and of which.
+struct PfCut {
+    PfItem item;
+    int pieces, len;                               // pieces of the item, 0: not a first piece; K / V tiles of each
+};
+
 struct PrefillArgs {
     __nv_bfloat16* out;
     float* part_o;                                 // pieces: [kPfPieces][2][128][D] sums of weights times values; NULL: nothing is cut
+    PfCut* cuts;                                   // [kPfPieces]
     float2* part_ml;                               // [kPfPieces][2][128]: maximum (log 2 units) and sum of the weights
     const __nv_bfloat16 *q, *k, *v;
     const int32_t *cu_q, *cu_k;
     int64_t o_ts, o_hs, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
     float scale_log2;
     int batch, q_tokens, kv_tokens, kv_heads, group, causal, out32;   // out32: rows of out are 32-byte aligned
-};
-
-struct PfItem {
-    int kv_row;                                    // first key of the sequence in k and v
-    int kv_len, kv_head;
-    // per query tile: first row in q and out, valid rows (1 .. 128), keys that row 0 sees before clamping (row r sees limit + r
-    // when causal), head, K / V tiles.  n[0] < 0: no more items; n[1] == 0: one query tile only.  n[0] <= n[1] otherwise.
-    int q_row[2], rows[2], limit[2], head[2], n[2];
-    int first;                                     // first K / V tile: 0 unless this is a piece of a cut item
-    int slot;                                      // where a piece leaves its result; < 0: a whole item, written to out
+    int packed;                                    // query rows of a tile that holds all heads of a group, or 0
+    PfDivide by_packed, by_group, by_kv_heads;
 };
 
 // Shared-memory matrix descriptors, as two words so that a step along an operand is one 32-bit addition.  High word: 1024
@@ -184,7 +213,7 @@ template <int N> __device__ __forceinline__ void regs_down() { asm volatile("set
 
 struct PfBarriers {
     uint64_t item_full[2], item_empty[2], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], l_full[2];
-    uint64_t kv_full[10], kv_empty[10], v_raw, taken;
+    uint64_t kv_full[10], kv_empty[10], v_raw, taken, loads_end;
 };
 
 // A lane-0 wait broadcast to the warp: everybody agrees on whether it ran out.
@@ -193,48 +222,51 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { retu
 // The query tiles of a sequence and kv head - blocks of 128 rows, and for each the heads of the group - are numbered block by
 // block, heads first, and an item is two neighbours: mostly two heads on the same rows, which see the same keys.  A short
 // prompt then fills both tiles of an item (with 256 rows of one head per item, 64 prompts of 128 tokens took 69 us instead of 55).
+// Where that makes fewer tiles, a tile takes all heads of the group on 128 / group rows instead (packed).  At 40 / 8 heads
+// of 128, tiles by head only and with packed ones: 300 prompts of 17 tokens 235 and 78 us, 32 of 300 tokens 92 and 75, 16 times 4
+// new tokens over 4000 cached 165 and 62; one prompt of 200 tokens, where SMs are left over anyway, 11.7 and 12.4.
 // Items are handed out by their number of K / V tiles, most first, so that the last ones to start are short; among
 // equals sequence by sequence, kv heads fastest.  The lengths are only known on the device; a warp counts as it goes - the
 // numbers it is given only grow, so it keeps its place.
 struct PfSequence {
     int q0, n, k0, m;                              // first query row, query rows, first key, keys
-    __device__ __forceinline__ PfSequence(const PrefillArgs& p, int b) : q0(0), n(p.q_tokens), k0(0), m(p.kv_tokens) {
-        if (!p.cu_q) return;
-        const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
-        q0 = min(max(p.cu_q[b], 0), p.q_tokens);
-        n = min(max(p.cu_q[b + 1], q0), p.q_tokens) - q0;
-        k0 = min(max(cu_k[b], 0), p.kv_tokens);
-        m = min(max(cu_k[b + 1], k0), p.kv_tokens) - k0;
+    int rows, heads, tiles;                        // query rows of a block, tiles of a block (one per head, or one in all), tiles
+    __device__ __forceinline__ PfSequence(const PrefillArgs& p, int b) : q0(0), n(p.q_tokens), k0(0), m(p.kv_tokens), rows(kPfTile), heads(p.group) {
+        if (p.cu_q) {
+            const int32_t* cu_k = p.cu_k ? p.cu_k : p.cu_q;
+            q0 = min(max(p.cu_q[b], 0), p.q_tokens);
+            n = min(max(p.cu_q[b + 1], q0), p.q_tokens) - q0;
+            k0 = min(max(cu_k[b], 0), p.kv_tokens);
+            m = min(max(cu_k[b + 1], k0), p.kv_tokens) - k0;
+        }
+        tiles = (n + kPfTile - 1) / kPfTile * p.group;
+        if (p.packed == 0) return;
+        const int packed = p.by_packed(n + p.packed - 1);
+        if (packed < tiles) {
+            tiles = packed;
+            rows = p.packed;
+            heads = 1;
+        }
     }
-    __device__ __forceinline__ int tiles(const PrefillArgs& p) const { return (n + kPfTile - 1) / kPfTile * p.group; }
-    __device__ __forceinline__ int items(const PrefillArgs& p) const { return (tiles(p) + 1) / 2; }
+    __device__ __forceinline__ bool packed() const { return rows != kPfTile; }
+    __device__ __forceinline__ int items() const { return (tiles + 1) >> 1; }
+    __device__ __forceinline__ int block_of(const PrefillArgs& p, int tile) const { return heads == 1 ? tile : p.by_group(tile); }
     // Items (the last ones) with at least `cost` K / V tiles; an item that sees nothing counts as one tile.
     __device__ __forceinline__ int items_from(const PrefillArgs& p, int cost) const {
-        const int all = items(p), keys = (cost - 1) * kPfTile;     // such an item's last row sees more than `keys`
+        const int all = items(), keys = (cost - 1) * kPfTile;      // such an item's last row sees more than `keys`
         if (cost <= 1 || all == 0) return all;
         if (m <= keys) return 0;
         if (!p.causal) return all;
-        const int short_of = keys - (m - n);                       // the last row of block x sees m - n + min(n, 128 (x + 1)) keys
-        const int block = short_of < 0 ? 0 : min(short_of / kPfTile, (n - 1) / kPfTile);
-        return all - block * p.group / 2;                          // items whose second tile is in that block or a later one
+        const int short_of = keys - (m - n);                       // the last row of block x sees m - n + min(n, rows (x + 1)) keys
+        const int block = short_of < 0 ? 0 : (packed() ? p.by_packed(min(short_of, n - 1)) : min(short_of, n - 1) / kPfTile);
+        return all - (block * heads >> 1);                           // items whose second tile is in that block or a later one
     }
     // K / V tiles of the longest item, and of the shortest.
     __device__ __forceinline__ int longest() const { return n > 0 ? max(1, (m + kPfTile - 1) / kPfTile) : 0; }
     __device__ __forceinline__ int shortest(const PrefillArgs& p) const {
         if (!p.causal || n == 0) return longest();
-        const int block = p.group == 1 && n > kPfTile ? 1 : 0;     // of the first item's second query tile
-        return max(1, (min(m, m - n + min(n, (block + 1) * kPfTile)) + kPfTile - 1) / kPfTile);
-    }
-    // K / V tiles of all items together: the sum over c of items_from(c).
-    __device__ __forceinline__ int64_t work(const PrefillArgs& p) const {
-        const int64_t all = items(p), most = (m + kPfTile - 1) / kPfTile;
-        if (!p.causal || most <= 1) return all * max(most, (int64_t)1);
-        // items_from(c) = all - floor(k G / 2) with k = max(c - 1 - e, 0), e = ceil((m - n) / 128), for c = 2 .. most
-        const int64_t e = m >= n ? (m - n + kPfTile - 1) / kPfTile : -((n - m) / kPfTile), g = p.group;
-        auto sum = [&](int64_t x) {                                // of floor(k G / 2), k = 0 .. x
-            return x <= 0 ? (int64_t)0 : (g * (x * (x + 1) / 2) - ((g & 1) ? (x + 1) / 2 : 0)) / 2;
-        };
-        return all * most - (sum(most - 1 - e) - sum(e < 0 ? -e : 0));
+        const int block = heads == 1 && tiles > 1 ? 1 : 0;         // of the first item's second query tile
+        return max(1, (m - n + min(n, (block + 1) * rows) + kPfTile - 1) / kPfTile);
     }
 };
 struct PfOrder {
@@ -242,9 +274,17 @@ struct PfOrder {
     int below;                                     // the next lower cost that some item has
     int share;                                     // K / V tiles that would be every SM's equal part, or more than any item has
 
-    // Pieces of an item with c K / V tiles.  Only items of more than `share` are cut, into fewer than 2 c / share pieces, and all
-    // items together have at most share * kSmCount tiles: at most kPfPieces pieces, the first in the order.
-    __device__ __forceinline__ int pieces(int c) const { return c <= share + kPfSlack ? 1 : (c + share - 1) / share; }
+    bool full;                                     // there would be more than one piece per SM: round the number of an item's pieces down
+
+    // Pieces of an item with c K / V tiles, and the tiles of each but the last.  Only items of more than `share` are cut, into fewer
+    // than 2 c / share pieces, and all items together have at most share * kSmCount tiles: at most kPfPieces pieces, the first
+    // in the order.
+    __device__ __forceinline__ int piece_len(int c) const {
+        if (c <= share + kPfSlack) return c;
+        const int n = full ? c / share : (c + share - 1) / share;
+        return (c + n - 1) / n;
+    }
+    __device__ __forceinline__ int pieces(int c) const { const int len = piece_len(c); return len == c ? 1 : (c + len - 1) / len; }
 
     __device__ __forceinline__ void seat(const PrefillArgs& p, int c) {
         cost = c;
@@ -261,32 +301,34 @@ struct PfOrder {
         below = __reduce_max_sync(0xffffffffu, next);
     }
     __device__ __forceinline__ void start(const PrefillArgs& p) {
+        const int lane = threadIdx.x & 31;
         int most = 0;
-        int64_t all = 0;
-        for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
-            const PfSequence q(p, b);
-            most = max(most, q.longest());
-            all += q.work(p);
-        }
+        for (int b = lane; b < p.batch; b += 32) most = max(most, PfSequence(p, b).longest());
         share = 0x3fffffff;
+        full = false;
         if (p.part_o) {
+            int per = 1;                                           // lanes for a sequence, which share its costs
+            while (per * 2 * p.batch <= 32) per *= 2;
+            int64_t all = 0;                                       // K / V tiles of all items: the sum over c of items_from(c)
+            for (int b = lane / per; b < p.batch; b += 32 / per) {
+                const PfSequence q(p, b);
+                const int least = q.shortest(p);
+                if (lane % per == 0) all += (int64_t)q.items() * least;
+                for (int c = least + 1 + lane % per; c <= q.longest(); c += per) all += q.items_from(p, c);
+            }
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
             share = static_cast<int>(min(max((all * p.kv_heads + kSmCount - 1) / kSmCount, (int64_t)kPfMinPiece), (int64_t)0x3fffffff));
+            int big = 0;                                           // pieces of items that are not small beside the others
+            for (int b = lane / per; b < p.batch; b += 32 / per) {
+                const PfSequence q(p, b);
+                for (int c = max(q.shortest(p), share / 2 + 1) + lane % per; c <= q.longest(); c += per)
+                    big += (q.items_from(p, c) - q.items_from(p, c + 1)) * ((c + share - 1) / share);
+            }
+            full = __reduce_add_sync(0xffffffffu, big) * p.kv_heads > kSmCount;
         }
         base = 0;
         seat(p, __reduce_max_sync(0xffffffffu, most));
-    }
-    __device__ __forceinline__ int piece_len() const { return (cost + pieces(cost) - 1) / pieces(cost); }
-    // The which-th item that is cut, as its first piece.  False: there is no such item.
-    __device__ __forceinline__ bool find_cut(const PrefillArgs& p, int which, PfItem& it) {
-        int items = 0;                                             // of higher cost
-        while (cost > 0 && pieces(cost) > 1 && which >= items + count * p.kv_heads) {
-            items += count * p.kv_heads;
-            base += count * p.kv_heads * pieces(cost);
-            seat(p, below);
-        }
-        return cost > 0 && pieces(cost) > 1 && find(p, base + (which - items) * pieces(cost), it);
     }
     // The piece or item with this number.  False: there is none.
     __device__ __forceinline__ bool find(const PrefillArgs& p, int index, PfItem& it) {
@@ -296,9 +338,9 @@ struct PfOrder {
             seat(p, below);
         }
         if (cost <= 0) return false;
-        const int cut = pieces(cost), piece = (index - base) % cut, which = (index - base) / cut;
-        const int rank = which / p.kv_heads;
-        it.kv_head = which % p.kv_heads;
+        const int cut = pieces(cost), which = cut > 1 ? (index - base) / cut : index - base, piece = index - base - which * cut;
+        const int rank = p.by_kv_heads(which);
+        it.kv_head = which - rank * p.kv_heads;
         // the sequence whose share of this cost holds `rank`
         int mine, upto;
         for (;;) {
@@ -322,20 +364,21 @@ struct PfOrder {
         const int src = max(__ffs(holds) - 1, 0);
         const PfSequence q(p, min(chunk + src, p.batch - 1));
         const int in_share = rank - before - __shfl_sync(0xffffffffu, upto - mine, src);
-        const int item = q.items(p) - q.items_from(p, cost) + in_share, tiles = q.tiles(p);
+        const int item = q.items() - q.items_from(p, cost) + in_share, tiles = q.tiles;
         it.kv_row = q.k0;
         it.kv_len = q.m;
+        it.packed = q.packed();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int x = min(2 * item + t, tiles - 1), first = x / p.group * kPfTile;
-            it.head[t] = it.kv_head * p.group + x % p.group;
+            const int x = min(2 * item + t, tiles - 1), block = q.block_of(p, x), first = block * q.rows, rows = min(q.rows, q.n - first);
+            it.head[t] = it.kv_head * p.group + (x - block * q.heads);
             it.q_row[t] = q.q0 + first;
-            it.rows[t] = min(kPfTile, q.n - first);
+            it.rows[t] = it.packed ? rows * p.group : rows;
             it.limit[t] = p.causal ? first + 1 + (q.m - q.n) : q.m;
-            const int sees = p.causal ? min(q.m, it.limit[t] + it.rows[t] - 1) : q.m;
+            const int sees = p.causal ? it.limit[t] + rows - 1 : q.m;
             it.n[t] = 2 * item + t < tiles ? max(1, (sees + kPfTile - 1) / kPfTile) : 0;
         }
-        const int len = piece_len();
+        const int len = piece_len(cost);
         it.first = piece * len;
         it.slot = cut > 1 ? index : -1;
         if (cut > 1)
@@ -344,6 +387,16 @@ struct PfOrder {
         return holds != 0;
     }
 };
+
+// Query row and head of a tile's row, relative to the tile's first.
+__device__ __forceinline__ void row_of(const PrefillArgs& p, const PfItem& it, int r, int& row, int& head) {
+    row = r;
+    head = 0;
+    if (it.packed) {
+        row = p.by_group(r);
+        head = r - row * p.group;
+    }
+}
 
 // The grid has a CTA for every item, but only one per SM fits: a running CTA takes over the work of one that has not started
 // yet (cluster launch control), so the items go to whoever is free.  The answer is 16 bytes in shared memory.
@@ -403,8 +456,8 @@ __device__ __forceinline__ void redo_row(const PrefillArgs& p, int q_row, int he
 
 template <int D>
 __global__ void __launch_bounds__(kPfThreads, 1)
-sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                    const PrefillArgs p) {
+sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_packed, const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap, const PrefillArgs p) {
     using Shape = PfShape<D>;
     constexpr int ST = Shape::kStages;
     extern __shared__ __align__(1024) uint8_t smem_p[];
@@ -417,11 +470,12 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     const uint32_t q_smem = (smem_u32(smem_p) + 1023u) & ~1023u, ring = q_smem + 2 * Shape::kTileBytes;
     if (threadIdx.x == 0) {
         prefetch_map(&qmap);
+        prefetch_map(&qmap_packed);
         prefetch_map(&kmap);
         prefetch_map(&vmap);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.item_full[i], 1);
-            mbar_init(&bar.item_empty[i], 13);                     // warps 0-12
+            mbar_init(&bar.item_empty[i], 14);                     // warps 0-13
             mbar_init(&bar.q_full[i], 1);
             mbar_init(&bar.q_empty[i], 1);
             mbar_init(&bar.s_full[i], 1);
@@ -433,9 +487,16 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         }
         mbar_init(&bar.v_raw, 1);
         mbar_init(&bar.taken, 1);
+        mbar_init(&bar.loads_end, 1);
         for (int i = 0; i < ST; ++i) { mbar_init(&bar.kv_full[i], 1); mbar_init(&bar.kv_empty[i], 1); }
         mbar_init_fence();
     }
+    // A packed tile may have fewer than 128 rows: the rest, which no copy fills then, are zeros, not what was left there.
+    for (int x = threadIdx.x; p.packed > 0 && x < (kPfTile - p.packed * p.group) * 8 * Shape::kHalves * 2; x += kPfThreads) {
+        const int r = kPfTile - 1 - (x >> 3) / (2 * Shape::kHalves), h = (x >> 3) % (2 * Shape::kHalves);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(q_smem + h * 16384 + r * 128 + (x & 7) * 16), "r"(0u) : "memory");
+    }
+    fence_proxy_async_smem();
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -468,7 +529,9 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         for (int k = 0; next_item(k, it); ++k) {
             const int tiles = t == 0 ? it.n[0] : it.n[1];
             if (tiles == 0) continue;
-            const int sees = p.causal ? min(it.kv_len, (t == 0 ? it.limit[0] : it.limit[1]) + wq * 32 + lane) : it.kv_len;
+            int row, head;
+            row_of(p, it, wq * 32 + lane, row, head);
+            const int sees = p.causal ? min(it.kv_len, (t == 0 ? it.limit[0] : it.limit[1]) + row) : it.kv_len;
             float m = -INFINITY;                                   // M / c
             float2 l2 = make_float2(0.f, 0.f);
             bool ok = true;
@@ -544,14 +607,15 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 ok = warp_wait(&bar.l_full[t], phase) && warp_wait(&bar.o_full[t], phase);
                 if (!ok) continue;
                 tm_fence_after();
-                const int r = wq * 32 + lane, q_row = t == 0 ? it.q_row[0] : it.q_row[1], head = t == 0 ? it.head[0] : it.head[1];
-                const int limit = t == 0 ? it.limit[0] : it.limit[1];
+                const int r = wq * 32 + lane;
+                int row, head;
+                row_of(p, it, r, row, head);
                 const bool valid = r < (t == 0 ? it.rows[0] : it.rows[1]);
                 const float l = s_l[t][r];
-                const int sees = p.causal ? min(it.kv_len, limit + r) : it.kv_len;
+                const int sees = p.causal ? min(it.kv_len, (t == 0 ? it.limit[0] : it.limit[1]) + row) : it.kv_len;
                 const bool none = sees <= 0 || l == 0.f;           // nothing to average: zeros, whatever the product holds
                 const float2 inv2 = make_float2(1.f / l, 1.f / l);
-                __nv_bfloat16* dst = p.out + (int64_t)(q_row + r) * p.o_ts + (int64_t)head * p.o_hs;
+                __nv_bfloat16* dst = p.out + (int64_t)((t == 0 ? it.q_row[0] : it.q_row[1]) + row) * p.o_ts + (int64_t)((t == 0 ? it.head[0] : it.head[1]) + head) * p.o_hs;
                 float* part = p.part_o + (((size_t)max(it.slot, 0) * 2 + t) * kPfTile + r) * D;
                 uint32_t o_addr = tmem + lanes + 256 + t * kPfTile;
                 float2 odd2 = make_float2(0.f, 0.f);               // 0 x (a value that is not finite) is NaN
@@ -601,8 +665,10 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                 }
                 const bool odd = !none && valid && it.slot < 0 && odd2.x + odd2.y != 0.f;
                 for (uint32_t redo = __ballot_sync(0xffffffffu, odd && l < INFINITY); redo; redo &= redo - 1) {
-                    const int rr = wq * 32 + __ffs(redo) - 1;
-                    redo_row<D>(p, q_row + rr, head, it.kv_row, p.causal ? min(it.kv_len, limit + rr) : it.kv_len);
+                    int i, h;
+                    row_of(p, it, wq * 32 + __ffs(redo) - 1, i, h);
+                    redo_row<D>(p, (t == 0 ? it.q_row[0] : it.q_row[1]) + i, (t == 0 ? it.head[0] : it.head[1]) + h, it.kv_row,
+                                p.causal ? min(it.kv_len, (t == 0 ? it.limit[0] : it.limit[1]) + i) : it.kv_len);
                 }
             }
         }
@@ -684,59 +750,28 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         } else if (warp == 13) {
             // ---------------- producer ----------------
             uint32_t q_uses[2] = {0, 0}, kv = 0, v_raws = 0;
-            PfOrder order;
             PfItem it;
             bool ok = true;
-            auto load = [&](const CUtensorMap* map, int head, int row, uint32_t dst, uint64_t* full) {
+            const uint32_t packed_bytes = static_cast<uint32_t>(p.packed * p.group * D * 2);
+            auto load = [&](const CUtensorMap* map, int head, int row, uint32_t dst, uint64_t* full, uint32_t bytes = Shape::kTileBytes) {
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(full, Shape::kTileBytes);
+                    mbar_arrive_expect_tx(full, bytes);
 #pragma unroll
                     for (int h = 0; h < Shape::kHalves; ++h) tma_rows(dst + h * 16384, map, h * 64, head, row, full);
                 }
             };
-            auto publish = [&](int k) {
-                if (k >= 2) ok = warp_wait(&bar.item_empty[k & 1], static_cast<uint32_t>((k >> 1) - 1) & 1u);
-                if (ok && lane == 0) {
-                    s_item[k & 1] = it;
-                    mbar_arrive(&bar.item_full[k & 1]);
-                }
-                __syncwarp();
-            };
-            int k = 0, index = blockIdx.x, asked = 0;
-            order.start(p);
-            auto ask = [&] {
-                if (elect_one()) {
-                    mbar_arrive_expect_tx(&bar.taken, 16);
-                    ask_for_cta(&s_answer, &bar.taken);
-                }
-                ++asked;
-            };
-            auto answer = [&] {
-                if (!warp_wait(&bar.taken, static_cast<uint32_t>(asked - 1) & 1u)) return false;
-                index = cta_taken(&s_answer);
-                fence_proxy_async_smem();                          // this read before the next answer is written
-                __syncwarp();
-                return true;
-            };
-            while (ok && index >= 0) {
-                if (!order.find(p, index, it)) {                   // past the real number: take these CTAs out of the way too
-                    ask();
-                    ok = answer();
-                    continue;
-                }
-                publish(k++);
+            for (int k = 0; ok && next_item(k, it); ++k) {
                 const int n_max = max(it.n[0], it.n[1]);
                 auto load_q = [&](int t) {
                     if (it.n[t] == 0 || !ok) return;
                     if (q_uses[t] > 0) ok = warp_wait(&bar.q_empty[t], (q_uses[t] - 1) & 1u);
                     if (!ok) return;
                     ++q_uses[t];
-                    load(&qmap, it.head[t], it.q_row[t], q_smem + t * Shape::kTileBytes, &bar.q_full[t]);
+                    load(it.packed ? &qmap_packed : &qmap, it.head[t], it.q_row[t], q_smem + t * Shape::kTileBytes, &bar.q_full[t], it.packed ? packed_bytes : Shape::kTileBytes);
                 };
                 if (ok) load_q(0);
                 for (int i = 0; i < 2 * n_max && ok; ++i, ++kv) {
-                    // the next item is asked for when this one's last tiles go out, not earlier: whoever is free shall have it
-                    if (i == max(0, 2 * n_max - 4)) ask();
+                    if (n_max > kPfEager && i == 2 * n_max - 4 && elect_one()) mbar_arrive(&bar.loads_end);
                     const int st = static_cast<int>(kv % ST);
                     if (kv >= ST) ok = warp_wait(&bar.kv_empty[st], (kv / ST - 1) & 1u);
                     if (!ok) break;
@@ -762,18 +797,53 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                     }
                     if (i == 0) load_q(1);
                 }
-                ok = ok && answer();
             }
-            it.n[0] = -1;
-            if (ok) publish(k);
             // no copy may still be under way when the CTA gives up its shared memory
             if (lane == 0) {
                 for (uint32_t i = kv > ST ? kv - ST : 0; i < kv; ++i) mbar_wait(&bar.kv_full[i % ST], (i / ST) & 1u);
                 for (int t = 0; t < 2; ++t)
                     if (q_uses[t] > 0) mbar_wait(&bar.q_full[t], (q_uses[t] - 1) & 1u);
                 if (v_raws > 0) mbar_wait(&bar.v_raw, (v_raws - 1) & 1u);
-                if (asked > 0) mbar_wait(&bar.taken, static_cast<uint32_t>(asked - 1) & 1u);
             }
+        } else if (warp == 14) {
+            // ---------------- scheduler ----------------
+            PfOrder order;
+            PfItem it;
+            bool ok = true;
+            auto publish = [&](int k) {
+                if (k >= 2) ok = warp_wait(&bar.item_empty[k & 1], static_cast<uint32_t>((k >> 1) - 1) & 1u);
+                if (ok && lane == 0) {
+                    s_item[k & 1] = it;
+                    mbar_arrive(&bar.item_full[k & 1]);
+                }
+                __syncwarp();
+            };
+            order.start(p);
+            uint32_t asked = 0, ends = 0;
+            int k = 0, index = blockIdx.x;
+            while (ok && index >= 0) {
+                const bool have = order.find(p, index, it);        // otherwise past the real number: take these CTAs out of the way too
+                if (p.part_o && index < kPfPieces && lane == 0) {
+                    PfCut& cut = p.cuts[index];
+                    cut.item = it;
+                    cut.len = order.piece_len(order.cost);
+                    cut.pieces = have && it.slot >= 0 && it.first == 0 ? order.pieces(order.cost) : 0;
+                }
+                if (have) {
+                    publish(k++);
+                    if (ok && max(it.n[0], it.n[1]) > kPfEager) ok = warp_wait(&bar.loads_end, ends++ & 1u);
+                }
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&bar.taken, 16);
+                    ask_for_cta(&s_answer, &bar.taken);
+                }
+                ok = warp_wait(&bar.taken, asked++ & 1u) && ok;
+                if (ok) index = cta_taken(&s_answer);
+                fence_proxy_async_smem();                          // this read before the next answer is written
+                __syncwarp();
+            }
+            it.n[0] = -1;
+            if (ok) publish(k);
         }
     }
     tm_fence_before();
@@ -782,35 +852,32 @@ sdpa_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     pdl_trigger();
 }
 
-// Joins the pieces of the items that were cut: CTA (i, t, quarter) takes 32 rows of query tile t of the i-th such item; a warp
-// takes a row at a time, a lane D / 32 columns.  The order of items is worked out again, which is shorter than passing it
-// on would be.
+// Joins the pieces of the items that were cut: a first piece is followed by another one at least, so CTA (i, t, quarter) looks at
+// the numbers 2 i and 2 i + 1 and takes 32 rows of query tile t; a warp takes a row at a time, a lane D / 32 columns.
+// (With the cut items found over again in every CTA, instead of read from what the main launch left, 8 times 64 new tokens over
+// 4000 cached, 32 / 4 heads of 128, took 65 us, not 55.)
 constexpr int kPfJoinWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kPfJoinWarps * 32)
 sdpa_prefill_join_kernel(const PrefillArgs p) {
     constexpr int W = D / 64;
-    __shared__ PfItem s_it;
-    __shared__ int s_cut, s_len;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.y;
     pdl_wait();
-    if (warp == 0) {
-        PfOrder order;
-        PfItem it;
-        order.start(p);
-        const bool have = order.find_cut(p, blockIdx.x, it);
-        if (lane == 0) {
-            s_cut = have ? order.pieces(order.cost) : 0;
-            s_len = have ? order.piece_len() : 0;
-            s_it = it;
-        }
-    }
-    __syncthreads();
-    const PfItem& it = s_it;
-    const int cut = s_cut, len = s_len;
-    if (cut > 0 && it.n[t] > 0) {
+    const PfCut& one = p.cuts[2 * blockIdx.x + (p.cuts[2 * blockIdx.x].pieces > 0 ? 0 : 1)];
+    const PfItem& it = one.item;
+    const int cut = one.pieces, len = one.len;
+    // A launch whose waits ran out (counted) may have left an entry unwritten.
+    const bool sane = it.slot >= 0 && cut <= kPfPieces - it.slot && len > 0 && it.kv_len >= 0 && it.kv_len <= p.kv_tokens && it.kv_row >= 0 &&
+                      it.kv_row <= p.kv_tokens - it.kv_len && it.q_row[t] >= 0 && it.q_row[t] < p.q_tokens && it.rows[t] <= kPfTile && it.head[t] >= 0 &&
+                      it.head[t] < p.kv_heads * p.group;
+    if (cut > 0 && sane && it.n[t] > 0) {
         for (int r = blockIdx.z * 32 + warp; r < min(it.rows[t], static_cast<int>(blockIdx.z) * 32 + 32); r += kPfJoinWarps) {
-            const int sees = p.causal ? min(it.kv_len, it.limit[t] + r) : it.kv_len;
+            int q_row, head;
+            row_of(p, it, r, q_row, head);
+            const int sees = p.causal ? min(it.kv_len, it.limit[t] + q_row) : it.kv_len;
+            q_row += it.q_row[t];
+            head += it.head[t];
+            if (q_row >= p.q_tokens || head >= p.kv_heads * p.group) break;        // no entry says that (see above)
             // pieces past the last key that the row sees hold nothing of it (and may not have looked at this tile at all)
             const int n = min(cut, max(1, (sees + len * kPfTile - 1) / (len * kPfTile)));
             auto at = [&](int i) { return ((size_t)(it.slot + i) * 2 + t) * kPfTile + r; };
@@ -836,28 +903,31 @@ sdpa_prefill_join_kernel(const PrefillArgs p) {
             }
             const bool none = sees <= 0 || sum == 0.f;
             bool odd = false;
-            __nv_bfloat16* dst = p.out + (int64_t)(it.q_row[t] + r) * p.o_ts + (int64_t)it.head[t] * p.o_hs;
+            __nv_bfloat16* dst = p.out + (int64_t)q_row * p.o_ts + (int64_t)head * p.o_hs;
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 const float x = none ? 0.f : acc[e].x / sum, y = none ? 0.f : acc[e].y / sum;
                 odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
                 *reinterpret_cast<uint32_t*>(dst + e * 64 + lane * 2) = pack_bf16x2(x, y);
             }
-            if (__any_sync(0xffffffffu, odd) && sum < INFINITY) redo_row<D>(p, it.q_row[t] + r, it.head[t], it.kv_row, sees);
+            if (__any_sync(0xffffffffu, odd) && sum < INFINITY) redo_row<D>(p, q_row, head, it.kv_row, sees);
         }
     }
     pdl_trigger();
 }
 
+// Query rows of a tile that holds all heads of a group; 0: there is nothing to pack, or one row's heads are too many for a tile.
+static int64_t packed_rows(int64_t group) { return group > 1 && group <= kPfTile ? kPfTile / group : 0; }
+
 template <int D>
-static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, int items, cudaStream_t st) {
+static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& qpm, const CUtensorMap& km, const CUtensorMap& vm, const PrefillArgs& p, int items, cudaStream_t st) {
     auto kern = sdpa_prefill_kernel<D>;
     static std::atomic<uint64_t> allowed{0};
     allow_smem(kern, PfShape<D>::kSmem, allowed);
-    launch_kernel(kern, items + (p.part_o ? kPfPieces : 0), kPfThreads, PfShape<D>::kSmem, st, qm, km, vm, p);
+    launch_kernel(kern, items + (p.part_o ? kPfPieces : 0), kPfThreads, PfShape<D>::kSmem, st, qm, qpm, km, vm, p);
     if (p.part_o) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(kSmCount, 2, kPfTile / 32);             // a cut item has more than an SM's equal part: fewer than kSmCount of them
+        cfg.gridDim = dim3(kPfPieces / 2, 2, kPfTile / 32);
         cfg.blockDim = dim3(kPfJoinWarps * 32);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
@@ -869,11 +939,16 @@ static void launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const C
     }
 }
 
-// Items: two query tiles (128 rows of a head) of a sequence and kv head each.  As many as the batch can have (every sequence
-// may end in a partly filled block and an odd tile); CTAs past the real number find nothing to do.
+// Items: two query tiles of a sequence and kv head each.  As many as the batch can have (every sequence may end in a partly
+// filled block and an odd tile), by heads or packed, whichever is less - no sequence takes the way that makes more tiles;
+// CTAs past the real number find nothing to do.
 static int64_t prefill_items(int64_t batch, int64_t q_tokens, int64_t heads, int64_t kv_heads) {
-    const int64_t full = (q_tokens + kPfTile - 1) / kPfTile, blocks = q_tokens < full + batch - 1 ? q_tokens : full + batch - 1;
-    return (blocks * (heads / kv_heads) + (blocks < batch ? blocks : batch)) / 2 * kv_heads;
+    auto items = [&](int64_t rows, int64_t tiles) {                // blocks of `rows` query rows with that many tiles
+        const int64_t full = (q_tokens + rows - 1) / rows, blocks = q_tokens < full + batch - 1 ? q_tokens : full + batch - 1;
+        return (blocks * tiles + (blocks < batch ? blocks : batch)) / 2 * kv_heads;
+    };
+    const int64_t group = heads / kv_heads, rows = packed_rows(group), by_head = items(kPfTile, group);
+    return rows > 0 ? std::min(by_head, items(rows, 1)) : by_head;
 }
 // Whether some item can be worth cutting, from what the host knows: few items, and keys for at least two pieces.  One
 // sequence is known well enough to tell that its longest item is no more than an SM's equal part.
@@ -890,7 +965,7 @@ extern "C" {
 int64_t nmt_sdpa_prefill_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
     using namespace nmt;
     if (batch <= 0 || q_tokens <= 0 || kv_tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads) return 0;
-    return prefill_may_cut(batch, q_tokens, kv_tokens, heads, kv_heads) ? (int64_t)kPfPieces * 2 * kPfTile * (head_dim * 4 + 8) : 0;
+    return prefill_may_cut(batch, q_tokens, kv_tokens, heads, kv_heads) ? (int64_t)kPfPieces * (2 * kPfTile * (head_dim * 4 + 8) + (int64_t)sizeof(PfCut)) : 0;
 }
 
 int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
@@ -918,18 +993,21 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
     struct { const void* p; int64_t tokens, ts, heads, hs; } views[3] = {{q, q_tokens, q_ts, heads, q_hs},
                                                                        {none ? q : k, none ? 1 : kv_tokens, k_ts, none ? 1 : kv_heads, k_hs},
                                                                        {none ? q : v, none ? 1 : kv_tokens, v_ts, none ? 1 : kv_heads, v_hs}};
-    CUtensorMap maps[3];
-    for (int i = 0; i < 3; ++i) {
-        const auto& w = views[i];
+    const int64_t group = heads / kv_heads;
+    const bool can_pack = packed_rows(group) > 0;
+    CUtensorMap maps[4];                                               // the last: q again, the heads of a group on neighbouring rows
+    for (int i = 0; i < (can_pack ? 4 : 3); ++i) {
+        const auto& w = views[i % 3];
         const int64_t hs = w.heads > 1 ? w.hs : head_dim, ts = w.tokens > 1 ? w.ts : head_dim * w.heads;
         if ((w.heads > 1 && hs < 1) || (w.tokens > 1 && ts < 1)) return NMT_ERR_UNSUPPORTED;       // a broadcast view
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(w.heads), static_cast<cuuint64_t>(w.tokens)};
         const cuuint64_t strides[2] = {static_cast<cuuint64_t>(hs * 2), static_cast<cuuint64_t>(ts * 2)};
-        const cuuint32_t box[3] = {64, 1, kPfTile}, ones[3] = {1, 1, 1};
+        const cuuint32_t box[3] = {64, i == 3 ? static_cast<cuuint32_t>(group) : 1u, static_cast<cuuint32_t>(i == 3 ? packed_rows(group) : kPfTile)}, ones[3] = {1, 1, 1};
         if (encode(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(w.p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return NMT_ERR_UNSUPPORTED;
     }
+    if (!can_pack) maps[3] = maps[0];
     PrefillArgs p;
     p.out = static_cast<__nv_bfloat16*>(out);
     p.q = static_cast<const __nv_bfloat16*>(q); p.k = static_cast<const __nv_bfloat16*>(k); p.v = static_cast<const __nv_bfloat16*>(v);
@@ -937,14 +1015,17 @@ int nmt_sdpa_prefill_bf16(const void* q, int64_t q_ts, int64_t q_hs, const void*
     p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.batch = static_cast<int>(batch); p.q_tokens = static_cast<int>(q_tokens); p.kv_tokens = static_cast<int>(kv_tokens);
-    p.kv_heads = static_cast<int>(kv_heads); p.group = static_cast<int>(heads / kv_heads); p.causal = causal != 0;
+    p.kv_heads = static_cast<int>(kv_heads); p.group = static_cast<int>(group); p.causal = causal != 0;
+    p.packed = static_cast<int>(packed_rows(group));
+    p.by_packed = PfDivide::of(p.packed > 0 ? p.packed : 1); p.by_group = PfDivide::of(group); p.by_kv_heads = PfDivide::of(kv_heads);
     p.out32 = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && (q_tokens == 1 || o_ts % 16 == 0) && (heads == 1 || o_hs % 16 == 0);
     const bool cut = workspace && prefill_may_cut(batch, q_tokens, kv_tokens, heads, kv_heads);
     p.part_o = cut ? static_cast<float*>(workspace) : nullptr;
     p.part_ml = cut ? reinterpret_cast<float2*>(p.part_o + (size_t)kPfPieces * 2 * kPfTile * head_dim) : nullptr;
+    p.cuts = cut ? reinterpret_cast<PfCut*>(p.part_ml + (size_t)kPfPieces * 2 * kPfTile) : nullptr;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (head_dim == 128) launch_prefill<128>(maps[0], maps[1], maps[2], p, static_cast<int>(items), cs);
-    else launch_prefill<64>(maps[0], maps[1], maps[2], p, static_cast<int>(items), cs);
+    if (head_dim == 128) launch_prefill<128>(maps[0], maps[3], maps[1], maps[2], p, static_cast<int>(items), cs);
+    else launch_prefill<64>(maps[0], maps[3], maps[1], maps[2], p, static_cast<int>(items), cs);
     return finish_launch(cut ? 2 : 1);
 }
 

@@ -53,6 +53,14 @@ CASES = [
     ([3], [0], 4, 2, 128, False),
     ([4000], None, 2, 1, 128, True),
     ([17] * 300, None, 5, 1, 64, True),
+    # few rows of many heads: tiles that hold all heads of a group
+    ([1, 3, 26, 25, 51, 126], [400, 3, 26, 700, 129, 126], 10, 2, 128, True),
+    ([1, 3, 26, 25, 51, 126], [400, 2, 26, 700, 20, 126], 10, 2, 128, True),
+    ([33, 16, 17, 5], [40, 1000, 17, 0], 16, 2, 64, False),
+    ([4, 130, 300], None, 128, 1, 64, True),
+    ([4, 130, 300], None, 130, 2, 128, True),                         # 65 heads per group: a row of them is half a tile
+    ([2, 129], None, 129, 1, 128, True),                              # more heads than rows: not packed
+    ([140, 1000], None, 24, 2, 64, True),
 ]
 
 
