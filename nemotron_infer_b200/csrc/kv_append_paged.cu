@@ -10,6 +10,9 @@
 // is 16 bytes wide and neighbouring lanes touch neighbouring vectors.  A warp owns up to 64 items of ONE token, two per
 // lane with all four loads issued before the first use; the sequence search, the page lookup and the cosine / sine row
 // are then per warp, not per head.  32 items of one kind (K, V or Q) at a time: what a lane does is the same all over the warp.
+// Bound by HBM for prompts and by the chain search - page lookup - load - store for a step.  Measured: 32 new tokens, 40 / 8
+// heads of 128 with rotation, 2.9 us (a launch alone 1.8); 9 prompts of up to 1100 tokens with q, strided, 11.7 us (4.6 TB/s);
+// 16,384 tokens into an e4m3 cache 24 us (4.2 TB/s: half the bytes written, the conversions are the rest).
 #include "nmt_paged.cuh"
 
 namespace nmt {

@@ -123,3 +123,22 @@ def test_two_streams_at_once(ops):
     for i, want in enumerate(alone):
         for d, p in got[i]:
             assert torch.equal(d, want[0]) and torch.equal(p, want[1])
+
+
+@pytest.mark.parametrize("interleaved,rot", [(False, 128), (True, 64)])
+def test_keys_rotated_with_the_queries(ops, interleaved, rot):
+    """A prompt's keys passed behind the queries come out as they stand in the pages, bit for bit, and prompt attention takes both
+    as views."""
+    g = gen(7)
+    ns, heads, kv, dim, page = [70, 1, 200], 10, 2, 128, 16
+    table, num = pages_for(ns, page, g)
+    kc, vc = (torch.zeros(num, kv, page, dim, dtype=BF, device="cuda") for _ in range(2))
+    cu = torch.tensor([0, 70, 71, 271], dtype=torch.int32, device="cuda")
+    qkv = randn(g, 271, heads + 2 * kv, dim)
+    k, v = qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+    qk = ops.kv_append_paged(k, v, kc, vc, table, torch.tensor(ns, dtype=torch.int32, device="cuda"), cu, q=qkv[:, :heads + kv],
+                             rope=ops.rope_table(256, rot), interleaved=interleaved)
+    pages = torch.cat([torch.cat([kc[int(p)] for p in table[b, :-(-n // page)]], dim=1)[:, :n].transpose(0, 1) for b, n in enumerate(ns)])
+    assert torch.equal(qk[:, heads:], pages)
+    out = ops.sdpa_prefill(qk[:, :heads], qk[:, heads:], v, cu)
+    assert torch.equal(out, ops.sdpa_prefill(qk[:, :heads].contiguous(), pages, v.contiguous(), cu))
