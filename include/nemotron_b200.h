@@ -271,7 +271,8 @@ typedef struct nmt_paged_cache {
  *   rope       NULL: no rotation.  Else fp32 [rope_rows][rot_dim]: row p holds rot_dim / 2 cosines, then as many sines, of
  *              position p.  The first rot_dim entries of every head are turned in pairs, (a, b) -> (a cos - b sin,
  *              b cos + a sin): entries (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved != 0.  rot_dim % 16 == 0.
- *   q, q_out   bf16 [tokens][q_heads][head_dim], or both NULL; needs rope.  q_out may be q.
+ *   q, q_out   bf16 [tokens][q_heads][head_dim], or both NULL; needs rope.  q_out may be q; it shares no memory with k or v
+ *              (NMT_ERR_UNSUPPORTED: keys that are to be rotated behind the queries, as further heads, need a new q_out).
  * fp32 arithmetic, one rounding to the type that is stored; e4m3(x / scale) saturates at +-448, NaN stays NaN.
  * A token whose position, page id or rope row is out of range writes nothing and sets *err_flag (device int32, may be
  * NULL) to 1.  Two tokens never share a slot unless the page table makes two sequences share a page; then which of
@@ -310,7 +311,7 @@ int nmt_sdpa_decode_paged_bf16(const nmt_paged_cache* cache, const void* q, int6
  *              (elements, multiples of 8): a view of a joint projection's output, or of the caches of
  *              nmt_sdpa_decode_bf16.  head_dim 64 or 128, heads a multiple of kv_heads, scale positive and finite.
  * fp32 scores, statistics and sums; the weights are good to 2^-18 and rounded to bf16 once for the product with v.  What a
- * mask hides is never used, not even an infinity or a NaN in v.
+ * mask hides is never used, not even an infinity or a NaN in v.  out shares no memory with q, k or v (NMT_ERR_UNSUPPORTED).
  *   workspace  nmt_sdpa_prefill_workspace_bytes(...) bytes, 32-byte aligned, no initialisation; calls whose kernels may
  *              overlap need one each.  The size is 0 unless the keys of few queries may be worth cutting into pieces, one
  *              per SM (a few new tokens over a long prefix); NULL is always allowed and cuts nothing.

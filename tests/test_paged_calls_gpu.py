@@ -142,3 +142,24 @@ def test_keys_rotated_with_the_queries(ops, interleaved, rot):
     assert torch.equal(qk[:, heads:], pages)
     out = ops.sdpa_prefill(qk[:, :heads], qk[:, heads:], v, cu)
     assert torch.equal(out, ops.sdpa_prefill(qk[:, :heads].contiguous(), pages, v.contiguous(), cu))
+
+
+def test_in_place_beside_the_keys(ops):
+    """Queries turned in place in a buffer that they share with k and v: behind one another, and head by head."""
+    g = gen(8)
+    T, heads, dim, page = 33, 4, 64, 16
+    table, num = pages_for([T], page, g)
+    lens, cu, rope = torch.tensor([T], dtype=torch.int32, device="cuda"), torch.tensor([0, T], dtype=torch.int32, device="cuda"), ops.rope_table(64, dim)
+    x = randn(g, T, heads, 3, dim)
+    for q, k, v in ((x[:, :, 0], x[:, :, 1], x[:, :, 2]), randn(g, T, 3 * heads, dim).split(heads, dim=1)):
+        want, got = [], []
+        for place in (None, q):
+            kc, vc = (torch.zeros(num, heads, page, dim, dtype=BF, device="cuda") for _ in range(2))
+            r = ops.kv_append_paged(k, v, kc, vc, table, lens, cu, q=q, rope=rope, q_out=place)
+            (want if place is None else got).extend([r.clone(), kc, vc])
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(RuntimeError):                              # the keys among the heads that are turned in place
+        y = randn(g, T, 3 * heads, dim)
+        ops.kv_append_paged(y[:, heads:2 * heads], y[:, 2 * heads:], kc, vc, table, lens, cu, q=y[:, :2 * heads], rope=rope, q_out=y[:, :2 * heads])
+    with pytest.raises(RuntimeError):
+        ops.sdpa_prefill(q, k, v, out=q)

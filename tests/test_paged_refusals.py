@@ -156,3 +156,15 @@ def test_prefill(built_lib):
     assert size(4, 100, 20000, 40, 8, 128) > 0 and size(1, 1, 20000, 40, 8, 64) > 0
     assert prefill(L, T=1 << 31, T_k=1 << 31) == UNSUPPORTED
     assert L.nmt_launch_count() == before
+
+
+def test_results_that_share_memory_with_inputs(built_lib):
+    L = built_lib
+    before = L.nmt_launch_count()
+    for out in ("q", "k", "v"):
+        at = {"q": BUF, "k": BUF + (1 << 20), "v": BUF + (2 << 20)}
+        assert prefill(L, **at, out=at[out], kts=5120 if out == "k" else 1024, cu=None, batch=1, T=1, T_k=1) == UNSUPPORTED
+    # keys behind the queries, as further heads, rotated in place: the key heads are read by others meanwhile
+    rope = dict(rope=BUF + (1 << 24), rows=10, rot=128)
+    assert append(L, cache(), k=BUF + 40 * 256, kts=40 * 128, q=BUF, q_heads=48, q_out=BUF, **rope) == UNSUPPORTED
+    assert L.nmt_launch_count() == before
