@@ -12,7 +12,7 @@
 // are then per warp, not per head.  32 items of one kind (K, V or Q) at a time: what a lane does is the same all over the warp.
 // Bound by HBM for prompts and by the chain search - page lookup - load - store for a step.  Measured: 32 new tokens, 40 / 8
 // heads of 128 with rotation, 2.9 us (a launch alone 1.8); 9 prompts of up to 1100 tokens with q, strided, 11.7 us (4.6 TB/s);
-// 16,384 tokens into an e4m3 cache 24 us (4.2 TB/s: half the bytes written, the conversions are the rest).
+// 16,384 tokens without rotation into an e4m3 cache 20 us (5.0 TB/s).
 #include "nmt_paged.cuh"
 
 namespace nmt {
@@ -59,8 +59,8 @@ __device__ __forceinline__ void rotate_item(float (&a)[8], float (&b)[8], const 
 // all - comes out exactly, for two instructions per pair of elements (a division takes about ten each).  lo is positive
 // and never zero (hi is cut from a value just below 1 / s): an infinity stays one.
 __device__ __noinline__ uint2 quantize_by_division(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float s) {
-    return make_uint2(e4m3x2_rn(__fdiv_rn(x0, s), __fdiv_rn(x1, s)) | (e4m3x2_rn(__fdiv_rn(x2, s), __fdiv_rn(x3, s)) << 16),
-                      e4m3x2_rn(__fdiv_rn(x4, s), __fdiv_rn(x5, s)) | (e4m3x2_rn(__fdiv_rn(x6, s), __fdiv_rn(x7, s)) << 16));
+    return make_uint2(e4m3x4_rn(__fdiv_rn(x0, s), __fdiv_rn(x1, s), __fdiv_rn(x2, s), __fdiv_rn(x3, s)),
+                      e4m3x4_rn(__fdiv_rn(x4, s), __fdiv_rn(x5, s), __fdiv_rn(x6, s), __fdiv_rn(x7, s)));
 }
 struct Divisor {
     float s, hi, lo;
@@ -82,12 +82,14 @@ struct Divisor {
             q[2 * e] = w.x;
             q[2 * e + 1] = w.y;
         }
-        return make_uint2(e4m3x2_rn(q[0], q[1]) | (e4m3x2_rn(q[2], q[3]) << 16), e4m3x2_rn(q[4], q[5]) | (e4m3x2_rn(q[6], q[7]) << 16));
+        return make_uint2(e4m3x4_rn(q[0], q[1], q[2], q[3]), e4m3x4_rn(q[4], q[5], q[6], q[7]));
     }
 };
 
-template <int D, bool E4M3, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppendWarps * 32, 10)    // 48 registers: loads in flight count, 16,384 tokens into e4m3 25.8 -> 24.0 us
+// No rotation is a kernel of its own: bound by instructions, and a third of them fall away (16,384 tokens into e4m3 24.1 -> 20.1 us).
+enum Turn { kNoTurn, kHalves, kNeighbours };
+template <int D, bool E4M3, Turn TURN>
+__global__ void __launch_bounds__(kAppendWarps * 32, 10)    // 48 registers: loads in flight count, 16,384 tokens into e4m3 7 % faster than with 64
 kv_append_kernel(const AppendArgs p) {
     constexpr int IPH = D / 16;                                    // items per head
     pdl_wait();
@@ -102,13 +104,13 @@ kv_append_kernel(const AppendArgs p) {
     auto place = [&](int kind, int in, int& h, int& off_a, int& off_b, bool& turn) {
         h = in / IPH;
         const int j = in % IPH;
-        turn = kind != 1 && j * 16 < p.rot;
-        const int base = turn || kind == 1 ? 0 : p.rot, span = turn ? p.rot : D - base;       // the part of the head that it belongs to
+        turn = TURN != kNoTurn && kind != 1 && j * 16 < p.rot;
+        const int base = TURN == kNoTurn || turn || kind == 1 ? 0 : p.rot, span = turn ? p.rot : D - base;       // the part of the head that it belongs to
         off_a = base + (j * 8 - base / 2);
         off_b = off_a + span / 2;
     };
     auto kind_of = [&](int slot, int& in, bool& have) {
-        const int kind = slot < kv_slots ? 0 : slot < 2 * kv_slots ? 1 : 2;
+        const int kind = slot < kv_slots ? 0 : TURN == kNoTurn || slot < 2 * kv_slots ? 1 : 2;
         in = (slot - kind * kv_slots) * 32 + lane;
         have = in < (kind == 2 ? n_q : n_kv);
         return kind;
@@ -137,12 +139,12 @@ kv_append_kernel(const AppendArgs p) {
     const int64_t pg = pos >> p.page_shift;
     int page = -1;
     if (pos >= 0 && pg < p.max_pages) page = p.page_table[(int64_t)b * p.max_pages + pg];
-    if (page < 0 || page >= p.num_pages || (p.rope && pos >= p.rope_rows)) {
+    if (page < 0 || page >= p.num_pages || (TURN != kNoTurn && pos >= p.rope_rows)) {
         if (p.err_flag && lane == 0) *p.err_flag = 1;
         return;
     }
     const int slot = static_cast<int>(pos) & ((1 << p.page_shift) - 1);
-    const float* row = p.rope ? p.rope + pos * p.rot : nullptr;
+    const float* row = TURN != kNoTurn ? p.rope + pos * p.rot : nullptr;
 #pragma unroll
     for (int i = 0; i < kItemsPerLane; ++i) {
         int in, h, off_a, off_b;
@@ -155,9 +157,9 @@ kv_append_kernel(const AppendArgs p) {
             unpack8(va[i], a);
             unpack8(vb[i], c);
         }
-        if (turn) rotate_item<INTERLEAVED>(a, c, row, half, off_a, off_b);
+        if (turn) rotate_item<TURN == kNeighbours>(a, c, row, half, off_a, off_b);
         if (turn && (!E4M3 || kind == 2)) { va[i] = pack8(a); vb[i] = pack8(c); }
-        if (kind == 2) {
+        if (TURN != kNoTurn && kind == 2) {
             __nv_bfloat16* dst = p.q_out + t * p.qo_ts + h * p.qo_hs;
             st_stream(reinterpret_cast<uint4*>(dst + off_a), va[i]);
             st_stream(reinterpret_cast<uint4*>(dst + off_b), vb[i]);
@@ -222,14 +224,14 @@ int nmt_kv_append_paged_bf16(const nmt_paged_cache* c, const int32_t* cu_new, in
     if (ctas > 0x3fffffff / kAppendWarps) return NMT_ERR_UNSUPPORTED;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     const bool e4m3 = c->dtype == NMT_CACHE_E4M3;
-#define NMT_APPEND(D, E, I) launch_kernel(kv_append_kernel<D, E, I>, static_cast<int>(ctas), kAppendWarps * 32, 0, cs, p)
-#define NMT_APPEND_D(D)                                                                  \
-    do {                                                                                 \
-        if (e4m3) { if (interleaved) NMT_APPEND(D, true, true); else NMT_APPEND(D, true, false); } \
-        else { if (interleaved) NMT_APPEND(D, false, true); else NMT_APPEND(D, false, false); }    \
+#define NMT_APPEND(D, E, T) launch_kernel(kv_append_kernel<D, E, T>, static_cast<int>(ctas), kAppendWarps * 32, 0, cs, p)
+#define NMT_APPEND_T(D, E)                                                                                          \
+    do {                                                                                                            \
+        if (!rope) NMT_APPEND(D, E, kNoTurn); else if (interleaved) NMT_APPEND(D, E, kNeighbours); else NMT_APPEND(D, E, kHalves); \
     } while (0)
-    if (c->head_dim == 128) NMT_APPEND_D(128); else NMT_APPEND_D(64);
-#undef NMT_APPEND_D
+    if (c->head_dim == 128) { if (e4m3) NMT_APPEND_T(128, true); else NMT_APPEND_T(128, false); }
+    else { if (e4m3) NMT_APPEND_T(64, true); else NMT_APPEND_T(64, false); }
+#undef NMT_APPEND_T
 #undef NMT_APPEND
     return finish_launch(1);
 }

@@ -70,10 +70,11 @@ __device__ __forceinline__ int find_segment(const int32_t* __restrict__ cu, int 
     return lo - 1;
 }
 
-// Two fp32 values -> two e4m3 bytes (`lo` in the low byte): round to nearest even, saturating, NaN kept.
-__device__ __forceinline__ uint32_t e4m3x2_rn(float lo, float hi) {
+// Four fp32 values -> four e4m3 bytes (a in the low one): round to nearest even, saturating, NaN kept.
+__device__ __forceinline__ uint32_t e4m3x4_rn(float a, float b, float c, float d) {
     uint32_t r;
-    asm("{ .reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %1, %2; cvt.u32.u16 %0, t; }" : "=r"(r) : "f"(hi), "f"(lo));
+    asm("{ .reg .b16 t, u; cvt.rn.satfinite.e4m3x2.f32 t, %2, %1; cvt.rn.satfinite.e4m3x2.f32 u, %4, %3; mov.b32 %0, {t, u}; }"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
 
