@@ -23,8 +23,8 @@
 //   * Precision.  P is split into two bf16 terms (p = hi + lo, 16 bits) against a bf16 V.  e4m3 values and the query,
 //     scaled by a power of two per head, are exact in f16 and P keeps 11 bits there.  Scores, maxima, sums, output: fp32.
 // Measured at 40 / 8 heads of 128: 192 sequences of 4000 tokens 472 us (6.66 TB/s), one of 131,071 tokens 88 us (6.1 TB/s), 64
-// ragged ones of up to 8192 over an e4m3 cache 38 us (3.8 TB/s: twice the arithmetic per byte, and the units' starts and
-// ends), one of 512 tokens 7.6 us - two launches and one chain of dependent loads each.
+// ragged ones of up to 8192 over an e4m3 cache 38 us (5.4 us before the first tile is there, 3.6 for the join; 64 of 8192
+// tokens run at 6.3 TB/s), one of 512 tokens 7.6 us - two launches and one chain of dependent loads each.
 #include <type_traits>
 
 #include "nmt_paged.cuh"
